@@ -3,7 +3,7 @@
 // positions of a table far larger than the 256 MiB Infinity Cache, each position exactly
 // once, and write a 256-byte result vector per 16 reads.  Known bytes are printed; compare
 // with the counters of kernel `calib_gather`:
-//   hipcc --offload-arch=gfx950 -O3 -o calib_fetch tools/calib_fetch.hip
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o calib_fetch tools/calib_fetch.hip
 //   rocprofv3 --pmc FETCH_SIZE -- ./calib_fetch ;  rocprofv3 --pmc WRITE_SIZE -- ./calib_fetch
 #include <hip/hip_runtime.h>
 #include <cstdio>

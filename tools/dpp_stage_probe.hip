@@ -1,7 +1,7 @@
 // Diagnostic for the pieces of the candidate hit loop of gpr_idx_probe.hip, one wave, every value
 // dumped and compared on the host: (1) DPP row_newbcast on a 32-bit move, (2) DPP row_shl packing of
 // four bytes, (3) gradient rows staged global -> LDS with per-lane addresses and read back.
-//   hipcc -O3 --offload-arch=gfx950 -Wno-inline-asm -o tools/dpp_stage_probe tools/dpp_stage_probe.hip
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-inline-asm -o tools/dpp_stage_probe tools/dpp_stage_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

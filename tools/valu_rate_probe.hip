@@ -1,6 +1,6 @@
 // Instruction-rate probe for gfx950: what a SIMD spends on the pieces of a sparse hit update, with
 // every SIMD holding WPS waves that run the same register-only loop (no memory in the loop).
-//   hipcc -O3 --offload-arch=gfx950 -Wno-inline-asm -o tools/valu_rate_probe tools/valu_rate_probe.hip
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-inline-asm -o tools/valu_rate_probe tools/valu_rate_probe.hip
 // Prints ns per loop body per SIMD (= per wave body / waves per SIMD) for each body, and the ratio of
 // s_memtime to s_memrealtime ticks (the latter is a constant 100 MHz).
 #include <hip/hip_runtime.h>

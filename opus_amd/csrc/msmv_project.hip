@@ -66,6 +66,22 @@ __device__ __forceinline__ float proj_row(const float *M, float x, float y, floa
     return ((a + b) + c) + M[3];
 }
 
+// The same row for the backward, which divides by the depth twice: where cancellation leaves a depth near zero, each
+// rounding of the sum is magnified, up to several 1e-5 of the largest gradient.  So the order of the operations is
+// written out instead of left to the compiler: it is the one the tensor-op formulation's matrix product agrees with.
+__device__ __forceinline__ float proj_depth(const float *M, float x, float y, float z)
+{
+#pragma clang fp contract(off)
+    const float a = M[0] * x, c = M[2] * z;
+    return (__builtin_fmaf(M[1], y, a) + c) + M[3];
+}
+__device__ __forceinline__ float proj_row_fused(const float *M, float x, float y, float z)
+{
+#pragma clang fp contract(off)
+    const float b = M[1] * y;
+    return __builtin_fmaf(M[2], z, __builtin_fmaf(M[0], x, b)) + M[3];
+}
+
 __global__ void __launch_bounds__(256)
 msmv_project_pack_fwd(const float *__restrict__ pts, const float *__restrict__ sw,
                       const float *__restrict__ occ2img, ProjDims d,
@@ -121,9 +137,9 @@ msmv_project_pack_bwd(const float *__restrict__ dloc, const float *__restrict__ 
     int view = (int)roundf(loc[(size_t)idx * 3 + 2] * (float)(d.N - 1));
     view = min(max(view, 0), d.N - 1);
     const float *M = occ2img + ((size_t)ix.b * d.T * d.N + (size_t)ix.t * d.N + view) * 16;
-    const float cx = M[0] * x + M[1] * y + M[2] * z + M[3];
-    const float cy = M[4] * x + M[5] * y + M[6] * z + M[7];
-    const float cz = M[8] * x + M[9] * y + M[10] * z + M[11];
+    const float cx = proj_row_fused(M, x, y, z);
+    const float cy = proj_row_fused(M + 4, x, y, z);
+    const float cz = proj_depth(M + 8, x, y, z);
     const float hz = fmaxf(cz, d.eps);
     const float du = dloc[(size_t)idx * 3], dv = dloc[(size_t)idx * 3 + 1];
     // u = cx / hz / image_w, v = cy / hz / image_h
@@ -166,9 +182,9 @@ msmv_project_pack_bwd_shared(const float *__restrict__ dloc, const float *__rest
         int view = (int)roundf(loc[idx * 3 + 2] * (float)(d.N - 1));
         view = min(max(view, 0), d.N - 1);
         const float *M = occ2img + ((size_t)b * d.T * d.N + (size_t)t * d.N + view) * 16;
-        const float cx = M[0] * x + M[1] * y + M[2] * z + M[3];
-        const float cy = M[4] * x + M[5] * y + M[6] * z + M[7];
-        const float cz = M[8] * x + M[9] * y + M[10] * z + M[11];
+        const float cx = proj_row_fused(M, x, y, z);
+        const float cy = proj_row_fused(M + 4, x, y, z);
+        const float cz = proj_depth(M + 8, x, y, z);
         const float hz = fmaxf(cz, d.eps);
         const float du = dloc[idx * 3], dv = dloc[idx * 3 + 1];
         const float gcx = du / (hz * d.image_w), gcy = dv / (hz * d.image_h);

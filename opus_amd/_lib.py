@@ -1,4 +1,4 @@
-"""ctypes binding of libopus_msmv.so (declared in include/opus_msmv.h).
+"""ctypes binding of libopus_msmv.so (declared in include/opus_msmv.h and include/opus_dense.h).
 
 This replaces the reference's pybind11 module ``_msmv_sampling_cuda``
 (models/csrc/msmv_sampling/msmv_sampling.cpp:362-368): the same four operations, taken
@@ -79,6 +79,55 @@ SYMBOLS = {
                            + [ctypes.c_void_p]),
 }
 
+# element types and names of include/opus_dense.h
+DENSE_F32, DENSE_BF16, DENSE_F16 = 0, 1, 2
+DENSE_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+DENSE_NORMS = {"layer": 0, "rms": 1}
+DENSE_MAX_WIDTH = 16384
+
+
+class DenseDropout(ctypes.Structure):
+    """opus_dense_dropout_t"""
+    _fields_ = [("threshold", ctypes.c_uint), ("offset", ctypes.c_uint), ("seed", ctypes.c_ulonglong),
+                ("seed_ptr", ctypes.c_void_p)]
+
+
+class DenseNorm(ctypes.Structure):
+    """opus_dense_norm_t"""
+    _fields_ = [("type", ctypes.c_int), ("kind", ctypes.c_int), ("rows", ctypes.c_longlong),
+                ("width", ctypes.c_longlong), ("gate_rows", ctypes.c_longlong), ("eps", ctypes.c_float),
+                ("scale", ctypes.c_float), ("x", ctypes.c_void_p), ("block", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("post_weight", ctypes.c_void_p),
+                ("post_bias", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("dropout", ctypes.POINTER(DenseDropout))]
+
+
+class DenseNormGrads(ctypes.Structure):
+    """opus_dense_norm_grads_t"""
+    _fields_ = [(name, ctypes.c_void_p) for name in
+                ("dx", "dblock", "dweight", "dbias", "dpost_weight", "dpost_bias", "dgate")]
+
+
+# name -> (restype, argtypes); every symbol include/opus_dense.h declares
+_drop_p = ctypes.POINTER(DenseDropout)
+DENSE_SYMBOLS = {
+    "opus_dense_strerror": (ctypes.c_char_p, [ctypes.c_int]),
+    "opus_dense_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] + [ctypes.c_longlong] * 3),
+    "opus_dense_linear_forward": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_longlong] * 3
+                                  + [ctypes.c_int, _drop_p] + [ctypes.c_void_p] * 3
+                                  + [ctypes.c_size_t, ctypes.c_void_p]),
+    "opus_dense_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] + [ctypes.c_longlong] * 3),
+    "opus_dense_linear_backward": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_longlong] * 3
+                                   + [ctypes.c_int, _drop_p] + [ctypes.c_void_p] * 5
+                                   + [ctypes.c_size_t, ctypes.c_void_p]),
+    "opus_dense_norm_forward": (ctypes.c_int, [ctypes.POINTER(DenseNorm)] + [ctypes.c_void_p] * 4),
+    "opus_dense_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] + [ctypes.c_longlong] * 3),
+    "opus_dense_norm_backward": (ctypes.c_int, [ctypes.POINTER(DenseNorm)] + [ctypes.c_void_p] * 3
+                                 + [ctypes.POINTER(DenseNormGrads), ctypes.c_void_p, ctypes.c_size_t,
+                                    ctypes.c_void_p]),
+    "opus_dense_dropout": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_void_p] * 2 + [ctypes.c_longlong] * 2
+                           + [_drop_p] + [ctypes.c_void_p] * 2),
+}
+
 _lib = None
 
 
@@ -99,7 +148,7 @@ def load():
             lib = ctypes.CDLL(LIB_PATH)
         except OSError as e:            # missing libamdhip64 etc.
             raise ImportError(f"cannot load {LIB_PATH}: {e}") from e
-        for name, (restype, argtypes) in SYMBOLS.items():
+        for name, (restype, argtypes) in [*SYMBOLS.items(), *DENSE_SYMBOLS.items()]:
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -114,6 +163,11 @@ def strerror(code):
 def check(code, what):
     if code != OK:
         raise RuntimeError(f"{what}: {strerror(code)} (code {code})")
+
+
+def check_dense(code, what):
+    if code != OK:
+        raise RuntimeError(f"{what}: {load().opus_dense_strerror(code).decode()} (code {code})")
 
 
 def ptr_array(ptrs):

@@ -1,0 +1,192 @@
+// Shared by the dense operators (include/opus_dense.h): element types and vector access, the dropout generator,
+// activations, and the host-side launchers.
+#pragma once
+#include "../../include/opus_dense.h"
+#include "msmv_launch.h"
+
+#include <stdint.h>
+
+typedef __bf16 dn_bf16;
+typedef _Float16 dn_f16;
+
+// N elements of T in registers.  `at` is the same vector with T's own alignment: gfx950 takes global vector accesses
+// at any element address, so rows of odd length are loaded and stored in vectors too (an aligned address costs
+// nothing extra, an odd one a second cache line at times).
+template <class T, int N> struct DnVec {
+    typedef T type __attribute__((ext_vector_type(N)));
+    typedef T at __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <int N> using dn_floats = typename DnVec<float, N>::type;
+
+template <int N, class T> __device__ __forceinline__ typename DnVec<T, N>::type dn_load(const T *p)
+{
+    return *reinterpret_cast<const typename DnVec<T, N>::at *>(p);
+}
+template <int N, class T> __device__ __forceinline__ void dn_store(T *p, typename DnVec<T, N>::type v)
+{
+    *reinterpret_cast<typename DnVec<T, N>::at *>(p) = v;
+}
+
+// Up to N elements as floats: all N where `n` >= N, zeros beyond `n` otherwise.
+template <int N, class T> __device__ __forceinline__ dn_floats<N> dn_load_n(const T *p, int n)
+{
+    dn_floats<N> r = 0.f;
+    if (n >= N) {
+        r = __builtin_convertvector(dn_load<N>(p), dn_floats<N>);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < n)
+                r[j] = (float)p[j];
+    }
+    return r;
+}
+
+// The first `n` of N floats, each rounded to T once, to nearest even.
+template <int N, class T> __device__ __forceinline__ void dn_store_n(T *p, dn_floats<N> v, int n)
+{
+    const typename DnVec<T, N>::type r = __builtin_convertvector(v, typename DnVec<T, N>::type);
+    if (n >= N) {
+        dn_store<N>(p, r);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < n)
+                p[j] = r[j];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// dropout
+// ------------------------------------------------------------------------------------------------
+struct DnDrop {
+    uint32_t threshold;          // 0: no dropout
+    uint32_t offset;
+    float scale;                 // 65536 / (65536 - threshold); 0 where everything is dropped
+    uint64_t seed;
+    const uint64_t *seed_ptr;
+};
+
+__device__ __forceinline__ uint64_t dn_seed(const DnDrop &d)
+{
+    return d.threshold && d.seed_ptr ? *d.seed_ptr : d.seed;
+}
+
+// Philox 4x32-10 (Salmon, Moraes, Dror, Shaw, SC'11): ten rounds of two 32 x 32 -> 64-bit products.  The round keys
+// depend on the seed alone and stay in scalar registers.
+__device__ __forceinline__ void dn_philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint64_t seed,
+                                          uint32_t (&out)[4])
+{
+    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)p1;
+        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)p0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    out[0] = c0; out[1] = c1; out[2] = c2; out[3] = c3;
+}
+
+// D on N (4 or 8) consecutive elements of a row, the first at column `col`, a multiple of N.  16 bits an element:
+// one generator call serves eight, which keeps a 16-bit tensor's dropout bound by memory (with 32 bits an element
+// the ten rounds, about 480 cycles of a SIMD for 64 calls, would take longer than the bytes).  A dropped element is
+// selected away, not multiplied by zero: inf and NaN vanish with it.
+template <int N>
+__device__ __forceinline__ void dn_drop(dn_floats<N> &v, uint64_t row, uint32_t col, uint64_t seed, const DnDrop &d)
+{
+    uint32_t w[4];
+    dn_philox(col >> 3, (uint32_t)row, (uint32_t)(row >> 32), d.offset, seed, w);
+    if (N == 4 && (col & 4)) {
+        w[0] = w[2];
+        w[1] = w[3];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t bits = j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
+        v[j] = bits >= d.threshold ? v[j] * d.scale : 0.f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// activations (in fp32)
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float dn_relu(float z) { return z > 0.f ? z : (z != z ? z : 0.f); }
+__device__ __forceinline__ float dn_gelu(float z) { return 0.5f * z * (1.f + erff(z * 0.70710678f)); }
+// 0.5 z (1 + tanh u) = z / (1 + exp(-2u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
+__device__ __forceinline__ float dn_gelu_tanh(float z)
+{
+    return z / (1.f + expf(-1.59576912f * (z + 0.044715f * z * z * z)));
+}
+__device__ __forceinline__ float dn_silu(float z) { return z / (1.f + expf(-z)); }
+
+__device__ __forceinline__ float dn_gelu_slope(float z)
+{
+    return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+}
+// s = (1 + tanh u) / 2;  s + 2 z s (1 - s) u'
+__device__ __forceinline__ float dn_gelu_tanh_slope(float z)
+{
+    const float z2 = z * z, s = 1.f / (1.f + expf(-1.59576912f * (z + 0.044715f * z * z2)));
+    return s + 2.f * z * s * (1.f - s) * 0.79788456f * (1.f + 0.134145f * z2);
+}
+__device__ __forceinline__ float dn_silu_slope(float z)
+{
+    const float s = 1.f / (1.f + expf(-z));
+    return s * (1.f + z * (1.f - s));
+}
+
+// v[j] = act(v[j]); the choice is uniform and outside the loops
+template <int N> __device__ __forceinline__ void dn_act(dn_floats<N> &v, int act)
+{
+#define DN_EACH(expr) _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = expr
+    switch (act) {
+    case OPUS_DENSE_ACT_RELU: DN_EACH(dn_relu(v[j])); break;
+    case OPUS_DENSE_ACT_GELU: DN_EACH(dn_gelu(v[j])); break;
+    case OPUS_DENSE_ACT_GELU_TANH: DN_EACH(dn_gelu_tanh(v[j])); break;
+    case OPUS_DENSE_ACT_SILU: DN_EACH(dn_silu(v[j])); break;
+    default: break;
+    }
+}
+
+// v[j] *= act'(z[j])
+template <int N> __device__ __forceinline__ void dn_act_slope(dn_floats<N> &v, const dn_floats<N> &z, int act)
+{
+    switch (act) {
+    case OPUS_DENSE_ACT_RELU: DN_EACH(z[j] > 0.f ? v[j] : 0.f); break;
+    case OPUS_DENSE_ACT_GELU: DN_EACH(v[j] * dn_gelu_slope(z[j])); break;
+    case OPUS_DENSE_ACT_GELU_TANH: DN_EACH(v[j] * dn_gelu_tanh_slope(z[j])); break;
+    case OPUS_DENSE_ACT_SILU: DN_EACH(v[j] * dn_silu_slope(z[j])); break;
+    default: break;
+    }
+#undef DN_EACH
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+inline size_t dn_type_bytes(int type) { return type == OPUS_DENSE_F32 ? 4 : 2; }
+inline long long dn_ceil(long long a, long long b) { return (a + b - 1) / b; }
+
+// y = residual + D(x) (slope == NULL), or D(x) * act'(slope) (slope = z, residual NULL).
+hipError_t dn_launch_elementwise(int type, const void *x, const void *residual, const void *slope, int act,
+                                 long long rows, long long cols, const DnDrop &drop, void *y, hipStream_t s);
+
+hipError_t dn_launch_norm_forward(const opus_dense_norm_t &in, const DnDrop &drop, void *y, void *stream_out,
+                                  float *stats, hipStream_t s);
+size_t dn_norm_backward_workspace(long long rows, long long width, long long gate_rows);
+hipError_t dn_launch_norm_backward(const opus_dense_norm_t &in, const DnDrop &drop, const void *dy,
+                                   const void *dstream, const float *stats, const opus_dense_norm_grads_t &out,
+                                   float *workspace, hipStream_t s);
+
+size_t dn_linear_forward_workspace(int type, long long M, long long N, long long K);
+hipError_t dn_launch_linear_forward(int type, const void *x, const void *w, const void *bias, const void *residual,
+                                    long long M, long long N, long long K, int act, const DnDrop &drop, void *y,
+                                    void *z, float *workspace, hipStream_t s);
+size_t dn_linear_backward_workspace(int type, long long M, long long N, long long K);
+hipError_t dn_launch_linear_backward(int type, const void *dz, const void *x, const void *w, long long M,
+                                     long long N, long long K, void *dx, void *dw, void *db, float *workspace,
+                                     hipStream_t s);

@@ -1,0 +1,556 @@
+// linear:  z = x W^T + bias,  y = residual + D(act(z)), and its gradients dx = dz W, dW = dz^T x, dbias = sum dz.
+//
+// All three are one product C[i, j] = sum_r A(i, r) B(j, r); an operand lies in memory either with r running fastest
+// ("RC": x and W in the forward, dz in dx) or with i (j) running fastest (W in dx, both operands in dW).
+//
+// A workgroup makes a BM x BN tile of C.  128 bytes of r at a time (64 bf16 / fp16 or 32 fp32 values), both operands'
+// tiles go to LDS by 16-byte transfers straight from memory (global_load_lds), double-buffered: the next tile is on
+// its way while the matrix cores work on this one.  Where a base or a row is not 16-byte aligned, or r ends inside a
+// tile, the tile goes through registers instead, zeros filled in.
+//
+// In LDS a 16-byte piece of an RC tile's row `row` stands at position piece ^ ((row >> 1) & 7): 16 rows read at the
+// same piece hit all 64 banks.  The other kind of tile keeps memory's order of r rows; a wave reads its operands with
+// ds_read_b64_tr_b16, which hands a lane four values of r at one i (fp32: plain 4-byte reads), and pieces are moved
+// so that the rows of one read lie in different banks.
+//
+// Matrix instructions: 32 x 32 x 16 (16-bit types) and 32 x 32 x 2 (fp32), sums in fp32.  fp32 operands stay fp32.
+//
+// The epilogue turns a wave's 32-row strip of C round through LDS, so that a lane holds eight consecutive columns of
+// one row: 16-byte accesses to bias, residual, z and y, and one generator call of the dropout for the eight.  Few
+// tiles and a long r: r is cut up over workgroups, each stores its fp32 share, and a second kernel adds the shares in
+// order and runs the epilogue.  No atomics: the result does not depend on the order of the workgroups.
+#include "dense_common.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------------------------------------------------
+// epilogue
+// ------------------------------------------------------------------------------------------------
+struct Epilogue {
+    const void *bias, *residual;
+    void *y, *z;
+    int act;
+    DnDrop drop;
+};
+
+// v: eight values of C at (row, col ..), `n` of them inside; col is a multiple of 8.
+template <class T>
+__device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, uint64_t row, uint32_t col, int n,
+                                       uint32_t cols, uint64_t seed)
+{
+    const uint64_t at = row * cols + col;
+    if (e.bias)
+        v += dn_load_n<8>(static_cast<const T *>(e.bias) + col, n);
+    if (e.z) {
+        dn_floats<8> z = v;
+        // fp16: a tiny z must not become 0, or relu's gradient would take it for a negative one
+        if constexpr (sizeof(T) == 2)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if ((float)(T)z[j] == 0.f && z[j] > 0.f)
+                    z[j] = 6e-8f;
+        dn_store_n<8>(static_cast<T *>(e.z) + at, z, n);
+    }
+    dn_act<8>(v, e.act);
+    if (e.drop.threshold)
+        dn_drop<8>(v, row, col, seed, e.drop);
+    if (e.residual)
+        v += dn_load_n<8>(static_cast<const T *>(e.residual) + at, n);
+    dn_store_n<8>(static_cast<T *>(e.y) + at, v, n);
+}
+
+// ------------------------------------------------------------------------------------------------
+// tiles
+// ------------------------------------------------------------------------------------------------
+struct GemmArgs {
+    const void *a, *b;           // A(i, r), B(j, r)
+    long long I, J, R;
+    int tiles_i, tiles_j, splits, steps, steps_per_split;       // steps: tiles of 128 bytes along r
+    float *partial;              // [splits][I][pitch], where splits > 1
+    long long pitch;
+    float *colsum;               // [splits][I]: sum over r of A(i, r), NULL: not wanted
+    Epilogue e;
+};
+
+template <class T> struct Elem;
+template <> struct Elem<float> { static constexpr int PIECE = 4, STEP = 32; };
+template <> struct Elem<dn_bf16> { static constexpr int PIECE = 8, STEP = 64; };
+template <> struct Elem<dn_f16> { static constexpr int PIECE = 8, STEP = 64; };
+
+// position of 16-byte piece `c` in row `row` of an LDS tile
+__device__ __forceinline__ int place_rc(int row, int c) { return c ^ ((row >> 1) & 7); }
+template <class T, int W> __device__ __forceinline__ int place_ic(int r, int c)
+{
+    if constexpr (sizeof(T) == 2 && W >= 128)
+        return c ^ ((r & 3) << 2);              // four r rows of a transposing read: 64 bytes apart
+    else if constexpr (sizeof(T) == 2)
+        return c ^ ((r & 2) << 1);              // (a row of 128 bytes: its neighbour is in the other banks already)
+    else
+        return c ^ ((r & 4) << 1);              // rows r and r + 4 of a read: the two halves of the banks
+}
+
+// One operand's tile: W rows of C (i or j) x 128 bytes of r.
+template <class T, bool RC, int W>
+struct Tile {
+    static constexpr int PIECE = Elem<T>::PIECE, STEP = Elem<T>::STEP;
+    static constexpr int PIECES = W * 8;                             // 16-byte pieces
+    static constexpr int ROW = RC ? 8 : W / PIECE;                   // pieces a row of the LDS tile
+    static constexpr int BYTES = PIECES * 16;
+
+    // piece p of the tile -> its coordinates: `w` (first i or the i), `r`
+    static __device__ __forceinline__ void coords(int p, int &w, int &r)
+    {
+        const int row = p / ROW, pos = p % ROW;
+        if constexpr (RC) {
+            w = row;
+            r = place_rc(row, pos) * PIECE;
+        } else {
+            r = row;
+            w = place_ic<T, W>(row, pos) * PIECE;
+        }
+    }
+
+    // Straight to LDS.  Rows beyond `I` (columns, where !RC) fetch the last valid one: what they make of C is never
+    // stored.  `r0 + STEP <= R`, 16-byte aligned rows.
+    template <int THREADS>
+    static __device__ __forceinline__ void fetch(const T *base, long long w0, long long r0, long long I, long long R,
+                                                 char *lds, int wave, int lane)
+    {
+        static_assert(PIECES % THREADS == 0, "whole turns");
+#pragma unroll
+        for (int t = 0; t < PIECES / THREADS; ++t) {
+            const int first = t * THREADS + wave * 64;
+            int w, r;
+            coords(first + lane, w, r);
+            const T *src;
+            if constexpr (RC) {
+                const long long row = min(w0 + w, I - 1);
+                src = base + row * R + (r0 + r);
+            } else {
+                const long long col = min(w0 + w, I - PIECE);
+                src = base + (r0 + r) * I + col;
+            }
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                             (__attribute__((address_space(3))) void *)(lds + first * 16), 16, 0, 0);
+        }
+    }
+
+    // Through registers: any alignment, zeros outside.
+    template <int THREADS>
+    static __device__ __forceinline__ void copy(const T *base, long long w0, long long r0, long long I, long long R,
+                                                char *lds, int tid)
+    {
+#pragma unroll
+        for (int t = 0; t < PIECES / THREADS; ++t) {
+            const int p = t * THREADS + tid;
+            int w, r;
+            coords(p, w, r);
+            typename DnVec<T, PIECE>::type v = (T)0.f;
+            const long long i = w0 + w, rr = r0 + r;
+            const T *src = RC ? base + i * R + rr : base + rr * I + i;
+            const long long inside = RC ? (i < I ? R - rr : 0) : (rr < R ? I - i : 0);
+            if (inside >= PIECE) {
+                v = dn_load<PIECE>(src);
+            } else {
+#pragma unroll
+                for (int j = 0; j < PIECE; ++j)
+                    if (j < inside)
+                        v[j] = src[j];
+            }
+            *reinterpret_cast<typename DnVec<T, PIECE>::type *>(lds + p * 16) = v;
+        }
+    }
+
+    // A lane's operands of rows w .. w+31 (lane % 32) for k-group `ks` (of 4): RC order of r: pieces 2 ks + lane / 32.
+    static __device__ __forceinline__ typename DnVec<T, PIECE>::type frag(const char *lds, int w, int ks, int lane)
+    {
+        if constexpr (RC) {
+            const int row = w + (lane & 31);
+            return *reinterpret_cast<const typename DnVec<T, PIECE>::type *>(
+                lds + (row * 8 + place_rc(row, ks * 2 + (lane >> 5))) * 16);
+        } else if constexpr (sizeof(T) == 2) {
+            // 16 lanes transpose 4 r rows x 16 columns: lane q of the 16 points at row q / 4, columns 4 (q % 4) ..,
+            // and receives the four rows of column q
+            const int q = lane & 15;
+            const int r = ks * 16 + (lane >> 5) * 8 + (q >> 2);
+            const int col = w + ((lane >> 4) & 1) * 16 + (q & 3) * 4;
+            const int at = (place_ic<T, W>(r, col >> 3) * 8 + (col & 7)) * 2;       // (r + 4 has the same r & 3)
+            typedef __attribute__((address_space(3))) s16x4 *lp;
+            const char *p = lds + r * (W * 2) + at;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * W * 2));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(typename DnVec<T, 8>::type, v);
+        } else {
+            f32x4 v;
+            const int col = w + (lane & 31);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int r = ks * 8 + (lane >> 5) * 4 + t;
+                v[t] = *reinterpret_cast<const float *>(lds + r * (W * 4) + place_ic<T, W>(r, col >> 2) * 16 + (col & 3) * 4);
+            }
+            return v;
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c)
+{
+    // a lane's four values are four r of the eight of the group: any order serves, as long as A and B have the same
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+}
+
+constexpr int STRIP = 72;       // floats a row of a wave's strip in LDS: rows four apart then start 32 banks apart
+
+// WI x WJ waves, each MI x MJ blocks of 32 x 32.  DIRECT: bases and rows are 16-byte aligned.
+template <class T, bool ARC, bool BRC, int WI, int WJ, int MI, int MJ, bool DIRECT>
+__global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
+{
+    constexpr int THREADS = WI * WJ * 64, BM = WI * MI * 32, BN = WJ * MJ * 32, STEP = Elem<T>::STEP;
+    using TA = Tile<T, ARC, BM>;
+    using TB = Tile<T, BRC, BN>;
+    constexpr int STAGE = TA::BYTES + TB::BYTES;
+    constexpr int STRIPS = WI * WJ * 32 * STRIP * 4;
+    __shared__ __align__(128) char lds[2 * STAGE > STRIPS ? 2 * STAGE : STRIPS];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wi = wave / WJ, wj = wave % WJ;
+
+    // Workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, so that the tiles sharing an
+    // operand share an L2.
+    int id = blockIdx.x;
+    const int total = g.tiles_i * g.tiles_j * g.splits, per = total >> 3, rest = total & 7, xcd = id & 7;
+    id = xcd * per + min(xcd, rest) + (id >> 3);
+    const int split = id / (g.tiles_i * g.tiles_j);
+    id -= split * g.tiles_i * g.tiles_j;
+    // tiles in bands of eight tile rows, down each band's columns
+    const int band = id / (8 * g.tiles_j), high = min(8, g.tiles_i - band * 8);
+    const int in = id - band * 8 * g.tiles_j;
+    const int tj = in / high, ti = band * 8 + in % high;
+    const long long i0 = (long long)ti * BM, j0 = (long long)tj * BN;
+    const int s0 = split * g.steps_per_split, s1 = min(s0 + g.steps_per_split, g.steps);
+
+    const T *pa = static_cast<const T *>(g.a), *pb = static_cast<const T *>(g.b);
+    const auto stage = [&](int s, char *to) {
+        const long long r0 = (long long)s * STEP;
+        if (DIRECT && r0 + STEP <= g.R) {
+            TA::template fetch<THREADS>(pa, i0, r0, g.I, g.R, to, wave, lane);
+            TB::template fetch<THREADS>(pb, j0, r0, g.J, g.R, to + TA::BYTES, wave, lane);
+        } else {
+            TA::template copy<THREADS>(pa, i0, r0, g.I, g.R, to, tid);
+            TB::template copy<THREADS>(pb, j0, r0, g.J, g.R, to + TA::BYTES, tid);
+        }
+    };
+
+    f32x16 acc[MI][MJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MJ; ++j)
+            acc[i][j] = 0.f;
+    float sum[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+        sum[i] = 0.f;
+    const bool want_sum = !ARC && g.colsum && tj == 0 && wj == 0;
+
+    if (s0 < s1)
+        stage(s0, lds);
+    for (int s = s0; s < s1; ++s) {
+        const int buf = (s - s0) & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (s + 1 < s1)
+            stage(s + 1, lds + (buf ^ 1) * STAGE);
+        const char *la = lds + buf * STAGE, *lb = la + TA::BYTES;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            typename DnVec<T, Elem<T>::PIECE>::type fa[MI], fb[MJ];
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+                fa[i] = TA::frag(la, (wi * MI + i) * 32, ks, lane);
+#pragma unroll
+            for (int j = 0; j < MJ; ++j)
+                fb[j] = TB::frag(lb, (wj * MJ + j) * 32, ks, lane);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < MJ; ++j)
+                    acc[i][j] = mma(fa[i], fb[j], acc[i][j]);
+            if (!ARC && want_sum)
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int t = 0; t < Elem<T>::PIECE; ++t)
+                        sum[i] += (float)fa[i][t];
+        }
+    }
+
+    if (!ARC && want_sum)
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const float t = sum[i] + __shfl_xor(sum[i], 32);
+            const long long row = i0 + (wi * MI + i) * 32 + (lane & 31);
+            if (lane < 32 && row < g.I)
+                g.colsum[split * g.I + row] = t;
+        }
+
+    // ---- epilogue: a wave turns 32 rows x (32 MJ, at most 64) columns at a time through its own strip
+    constexpr int SJ = MJ < 2 ? MJ : 2, CPR = SJ * 4, RPT = 64 / CPR;
+    const uint64_t seed = dn_seed(g.e.drop);
+    float *strip = reinterpret_cast<float *>(lds) + wave * 32 * STRIP;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int jj = 0; jj < MJ; jj += SJ) {
+#pragma unroll
+            for (int j = 0; j < SJ; ++j)
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+                    strip[((t >> 2) * 8 + (lane >> 5) * 4 + (t & 3)) * STRIP + j * 32 + (lane & 31)] = acc[i][jj + j][t];
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < 32 / RPT; ++q) {
+                const int row = q * RPT + lane / CPR, col = (lane % CPR) * 8;
+                const f32x4 lo = *reinterpret_cast<const f32x4 *>(strip + row * STRIP + col);
+                const f32x4 hi = *reinterpret_cast<const f32x4 *>(strip + row * STRIP + col + 4);
+                const long long ci = i0 + (wi * MI + i) * 32 + row, cj = j0 + (wj * MJ + jj) * 32 + col;
+                const dn_floats<8> v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                if (ci < g.I && cj < g.J) {
+                    if (g.partial)
+                        *reinterpret_cast<dn_floats<8> *>(g.partial + (split * g.I + ci) * g.pitch + cj) = v;
+                    else
+                        finish<T>(g.e, v, ci, (uint32_t)cj, (int)min(8ll, g.J - cj), (uint32_t)g.J, seed);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+// Adds the shares of r in order and runs the epilogue; a thread takes eight columns of a row.
+template <class T>
+__global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g)
+{
+    const uint64_t seed = dn_seed(g.e.drop);
+    const uint32_t units = (uint32_t)(g.pitch / 8);
+    const uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t row = u / units;
+    const uint32_t col = (uint32_t)(u - row * units) * 8;
+    if (row >= (uint64_t)g.I)
+        return;
+    dn_floats<8> v = 0.f;
+    const float *p = g.partial + row * g.pitch + col;
+    for (int s = 0; s < g.splits; ++s, p += g.I * g.pitch)
+        v += *reinterpret_cast<const dn_floats<8> *>(p);
+    finish<T>(g.e, v, row, col, (int)min((long long)8, g.J - (long long)col), (uint32_t)g.J, seed);
+}
+
+// dbias from the shares of the column sums
+template <class T>
+__global__ void __launch_bounds__(256) dense_colsum_join_kernel(const float *part, int splits, long long n, T *out)
+{
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n)
+        return;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k)
+        s += part[k * n + i];
+    out[i] = (T)s;
+}
+
+// Column sums of dz [M, N] by themselves (where dW is not wanted, or has no elements): 32 columns a workgroup
+// and a run of rows, which the kernel above adds.
+template <class T>
+__global__ void __launch_bounds__(256) dense_colsum_kernel(const T *dz, long long M, long long N, long long rows_per, float *part)
+{
+    __shared__ float lds[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const long long col = (long long)blockIdx.x * 32 + x, first = blockIdx.y * rows_per, last = min(first + rows_per, M);
+    float s = 0.f;
+    if (col < N)
+        for (long long m = first + y; m < last; m += 8)
+            s += (float)dz[m * N + col];
+    lds[y][x] = s;
+    __syncthreads();
+    if (y == 0 && col < N) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k)
+            s += lds[k][x];
+        part[blockIdx.y * N + col] = s;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+constexpr int CUS = 256;
+
+struct Plan {
+    int tile;                    // 0: 64 x 64, 1: 128 x 128
+    int tiles_i, tiles_j, splits, steps, steps_per_split;
+    long long pitch;
+    size_t bytes;                // of the fp32 shares
+};
+
+Plan plan(int type, long long I, long long J, long long R)
+{
+    Plan p = {};
+    p.splits = 1;
+    if (I < 1 || J < 1)
+        return p;
+    p.steps = (int)dn_ceil(R, type == OPUS_DENSE_F32 ? 32 : 64);
+    const long long big = dn_ceil(I, 128) * dn_ceil(J, 128);
+    p.tile = big >= CUS / 2 || (I > 64 && J > 64 && big * p.steps >= 4 * CUS) ? 1 : 0;
+    const int edge = p.tile ? 128 : 64;
+    p.tiles_i = (int)dn_ceil(I, edge);
+    p.tiles_j = (int)dn_ceil(J, edge);
+    const long long tiles = (long long)p.tiles_i * p.tiles_j;
+    // cut r until there are two workgroups a CU, but leave each at least four steps
+    long long splits = tiles >= CUS ? 1 : dn_ceil(2 * CUS, tiles);
+    if (splits > p.steps / 4)
+        splits = p.steps / 4;
+    if (splits < 1)
+        splits = 1;
+    p.steps_per_split = (int)dn_ceil(p.steps > 0 ? p.steps : 1, splits);
+    p.splits = p.steps > 0 ? (int)dn_ceil(p.steps, p.steps_per_split) : 1;
+    p.pitch = dn_ceil(J, 8) * 8;
+    p.bytes = p.splits > 1 ? (size_t)p.splits * I * p.pitch * sizeof(float) : 0;
+    return p;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <class T, bool ARC, bool BRC, bool DIRECT>
+void launch_tiles(const Plan &p, const GemmArgs &g, hipStream_t s)
+{
+    const dim3 grid((unsigned)(p.tiles_i * p.tiles_j * p.splits));
+    if (p.tile)
+        hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 2, 2, 2, DIRECT>), grid, dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 2, 1, 1, DIRECT>), grid, dim3(256), 0, s, g);
+}
+
+// C = A B^T with an epilogue; `shares`: p.bytes of workspace.  colsum: [p.splits][I] fp32 or NULL.
+template <class T, bool ARC, bool BRC>
+hipError_t gemm(int type, const void *a, const void *b, long long I, long long J, long long R, const Epilogue &e,
+                float *shares, float *colsum, hipStream_t s)
+{
+    const Plan p = plan(type, I, J, R);
+    if ((long long)p.tiles_i * p.tiles_j * p.splits * 256 > 0xFFFFFFFFll)
+        return hipErrorInvalidValue;
+    GemmArgs g = {a, b, I, J, R, p.tiles_i, p.tiles_j, p.splits, p.steps, p.steps_per_split,
+                  p.splits > 1 ? shares : nullptr, p.pitch, colsum, e};
+    const int piece = Elem<T>::PIECE;
+    const bool direct = aligned16(a) && aligned16(b) && (ARC ? R : I) % piece == 0 && (BRC ? R : J) % piece == 0;
+    if (direct)
+        launch_tiles<T, ARC, BRC, true>(p, g, s);
+    else
+        launch_tiles<T, ARC, BRC, false>(p, g, s);
+    if (p.splits > 1) {
+        const long long blocks = dn_ceil(I * (p.pitch / 8), 256);
+        if (blocks * 256 > 0xFFFFFFFFll)
+            return hipErrorInvalidValue;
+        hipLaunchKernelGGL(dense_gemm_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, g);
+    }
+    return hipSuccess;
+}
+
+// runs of rows of dense_colsum_kernel
+long long colsum_runs(long long M, long long N)
+{
+    const long long want = dn_ceil(4 * CUS, dn_ceil(N, 32)), most = dn_ceil(M, 64);
+    const long long runs = want < most ? want : most;
+    return runs < 1 ? 1 : runs > 65535 ? 65535 : runs;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+template <class T>
+hipError_t backward(int type, const void *dz, const void *x, const void *w, long long M, long long N, long long K,
+                    void *dx, void *dw, void *db, float *ws, hipStream_t s)
+{
+    hipError_t e = hipSuccess;
+    if (dx && M && K) {
+        const Epilogue ep = {nullptr, nullptr, dx, nullptr, OPUS_DENSE_ACT_NONE, {}};
+        e = gemm<T, true, false>(type, dz, w, M, K, N, ep, ws, nullptr, s);
+    }
+    if (e != hipSuccess)
+        return e;
+    const Plan p = plan(type, N, K, M);
+    float *sums = ws + align256(p.bytes) / sizeof(float);
+    if (dw && N && K) {
+        const Epilogue ep = {nullptr, nullptr, dw, nullptr, OPUS_DENSE_ACT_NONE, {}};
+        e = gemm<T, false, false>(type, dz, x, N, K, M, ep, ws, db ? sums : nullptr, s);
+        if (e != hipSuccess)
+            return e;
+        if (db)
+            hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 256)), dim3(256), 0, s, sums,
+                               p.splits, N, static_cast<T *>(db));
+    } else if (db && N) {
+        const long long runs = colsum_runs(M, N), per = dn_ceil(M > 0 ? M : 1, runs);
+        hipLaunchKernelGGL(dense_colsum_kernel<T>, dim3((unsigned)dn_ceil(N, 32), (unsigned)runs), dim3(256), 0, s,
+                           static_cast<const T *>(dz), M, N, per, ws);
+        hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 256)), dim3(256), 0, s, ws,
+                           (int)runs, N, static_cast<T *>(db));
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+size_t dn_linear_forward_workspace(int type, long long M, long long N, long long K)
+{
+    return M > 0 && N > 0 ? plan(type, M, N, K).bytes : 0;
+}
+
+hipError_t dn_launch_linear_forward(int type, const void *x, const void *w, const void *bias, const void *residual,
+                                    long long M, long long N, long long K, int act, const DnDrop &drop, void *y,
+                                    void *z, float *workspace, hipStream_t s)
+{
+    if (M == 0 || N == 0)
+        return hipSuccess;
+    const Epilogue e = {bias, residual, y, z, act, drop};
+    const hipError_t stale = hipPeekAtLastError();
+    const hipError_t r = type == OPUS_DENSE_F32 ? gemm<float, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s)
+                       : type == OPUS_DENSE_BF16 ? gemm<dn_bf16, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s)
+                                                 : gemm<dn_f16, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s);
+    return r != hipSuccess ? r : msmv_launch_status(stale);
+}
+
+size_t dn_linear_backward_workspace(int type, long long M, long long N, long long K)
+{
+    if (N <= 0)
+        return 0;
+    const size_t x = M > 0 && K > 0 ? plan(type, M, K, N).bytes : 0;
+    const Plan p = plan(type, N, K, M);
+    const size_t w = align256(p.bytes) + (size_t)p.splits * N * sizeof(float);
+    const size_t alone = (size_t)colsum_runs(M, N) * N * sizeof(float);
+    const size_t most = x > w ? x : w;
+    return most > alone ? most : alone;
+}
+
+hipError_t dn_launch_linear_backward(int type, const void *dz, const void *x, const void *w, long long M,
+                                     long long N, long long K, void *dx, void *dw, void *db, float *workspace,
+                                     hipStream_t s)
+{
+    const hipError_t stale = hipPeekAtLastError();
+    const hipError_t r = type == OPUS_DENSE_F32 ? backward<float>(type, dz, x, w, M, N, K, dx, dw, db, workspace, s)
+                       : type == OPUS_DENSE_BF16 ? backward<dn_bf16>(type, dz, x, w, M, N, K, dx, dw, db, workspace, s)
+                                                 : backward<dn_f16>(type, dz, x, w, M, N, K, dx, dw, db, workspace, s);
+    return r != hipSuccess ? r : msmv_launch_status(stale);
+}

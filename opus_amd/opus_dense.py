@@ -1,0 +1,351 @@
+"""The dense operators a decoder layer runs around ``sampling_4d``, as hand-written kernels with gradients.
+
+    linear          y = residual + D(act(x W^T + bias))
+    residual_norm   r = residual_scale * x + gate * D(post(block));  y = norm(r)
+    dropout         y = residual + D(x)
+
+The reference composes them from library layers (models/opus_transformer.py:225-247, :329-358, :381-448): the
+products that make sampling offsets and scale weights, the mixing's parameters and its way back into the query stream,
+the feed-forward block, and the norm that follows each of them.
+
+Common to the three: tensors are fp32, bf16 or fp16, all of one type, on one GPU (CPU tensors raise); products, sums,
+statistics and the epilogue are in fp32 and every result is rounded once.  A tensor that is not contiguous is copied
+first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep no
+state and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
+inputs give the same bits.  Gradients are first-order only.
+
+``D`` is dropout with a counter-based generator: whether element (row, column) is kept is computed from
+``(seed, offset, row, column)`` - row counting the tensor's last-dimension rows - by Philox 4x32-10, in the forward
+and again in the backward; no mask is stored, and the type, the operator and the launch make no difference to it.  The
+probability ``p`` is taken to the nearest multiple of 1/65536, kept elements are scaled by the inverse of the
+probability so rounded, and a dropped element is exactly 0 (even inf or NaN).  ``seed`` is an int (64 bits are used)
+or a one-element int64 tensor on the tensors' device, read when the kernels run: a captured graph draws new masks
+when that tensor is changed between replays.  It must not change between a forward and its backward.  Give every
+dropout of a step an ``offset`` (0 .. 2**32 - 1) of its own.
+"""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_TYPES = {torch.float32: _lib.DENSE_F32, torch.bfloat16: _lib.DENSE_BF16, torch.float16: _lib.DENSE_F16}
+
+
+# ------------------------------------------------------------------------------------------------
+# arguments
+# ------------------------------------------------------------------------------------------------
+def _check(what, x, others):
+    """One type, one GPU; ``others`` maps names to tensors or None."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: expected CUDA tensors")
+    if x.dtype not in _TYPES:
+        raise RuntimeError(f"{what}: expected float32, bfloat16 or float16 tensors, got {x.dtype}")
+    if x.dim() < 1:
+        raise RuntimeError(f"{what}: expected a tensor of at least one dimension")
+    for name, t in others:
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise RuntimeError(f"{what}: {name} is {t.dtype}, expected {x.dtype}")
+        if t.device != x.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, expected {x.device}")
+
+
+def _threshold(what, p, seed, offset, device):
+    """p -> threshold of 65536 (0: no dropout); checks the generator's arguments."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{what}: dropout probability has to be between 0 and 1, got {p}")
+    threshold = round(p * 65536)
+    if threshold == 0:
+        return 0
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+            raise RuntimeError(f"{what}: a seed tensor has to hold one int64 on {device}")
+    elif not isinstance(seed, int) or isinstance(seed, bool):
+        raise RuntimeError(f"{what}: dropout needs a seed, an int or a one-element int64 tensor")
+    if not 0 <= offset < 2 ** 32:
+        raise ValueError(f"{what}: offset has to be in [0, 2**32), got {offset}")
+    return threshold
+
+
+def _drop_struct(threshold, seed, offset):
+    if threshold == 0:
+        return None
+    if isinstance(seed, torch.Tensor):
+        return _lib.DenseDropout(threshold, offset, 0, seed.data_ptr())
+    return _lib.DenseDropout(threshold, offset, seed & (2 ** 64 - 1), None)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _run(what, fn, device, *args):
+    """Calls a C entry, whose last argument is the stream, with ``device`` current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc != 0:
+        _lib.check_dense(rc, what)
+
+
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------------------------------------
+# linear
+# ------------------------------------------------------------------------------------------------
+def _linear_forward(x, weight, bias, residual, activation, threshold, seed, offset, want_z):
+    lib = _lib.load()
+    N, K = weight.shape
+    shape = x.shape[:-1] + (N,)
+    x, weight, bias, residual = _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual)
+    M = x.numel() // K if K else shape.numel() // max(N, 1)
+    kind = _TYPES[x.dtype]
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(shape, dtype=x.dtype, device=x.device) if want_z else None
+    need = lib.opus_dense_linear_workspace_bytes(kind, M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _run("linear", lib.opus_dense_linear_forward, x.device, kind, x.data_ptr(), weight.data_ptr(), _ptr(bias),
+         _ptr(residual), M, N, K, activation, _drop_struct(threshold, seed, offset), y.data_ptr(), _ptr(z), _ptr(ws),
+         need)
+    return y, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, threshold, seed, offset):
+        y, z = _linear_forward(x, weight, bias, residual, activation, threshold, seed, offset, activation != 0)
+        seed_tensor = seed if isinstance(seed, torch.Tensor) and threshold else None
+        ctx.save_for_backward(x, weight, z, seed_tensor)
+        ctx.settings = activation, threshold, None if seed_tensor is not None else seed, offset
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, z, seed_tensor = ctx.saved_tensors
+        activation, threshold, seed, offset = ctx.settings
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            lib = _lib.load()
+            N, K = weight.shape
+            shape, kind, device = x.shape, _TYPES[x.dtype], x.device
+            x, weight, g = _contiguous(x), _contiguous(weight), _contiguous(dy)
+            M = x.numel() // K if K else dy.numel() // max(N, 1)
+            if need_x:
+                dx = torch.empty(shape, dtype=x.dtype, device=device)
+            if need_w:
+                dw = torch.empty((N, K), dtype=x.dtype, device=device)
+            if need_b:
+                db = torch.empty((N,), dtype=x.dtype, device=device)
+            dz = torch.empty_like(g) if activation or threshold else None
+            need = lib.opus_dense_linear_backward_workspace_bytes(kind, M, N, K)
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            _run("linear backward", lib.opus_dense_linear_backward, device, kind, g.data_ptr(), x.data_ptr(),
+                 weight.data_ptr(), _ptr(z), M, N, K, activation,
+                 _drop_struct(threshold, seed if seed_tensor is None else seed_tensor, offset), _ptr(dz), _ptr(dx),
+                 _ptr(dw), _ptr(db), _ptr(ws), need)
+        return dx, dw, db, dy if need_r else None, None, None, None, None
+
+
+def linear(x, weight, bias=None, activation="none", residual=None, dropout_p=0.0, seed=None, offset=0):
+    """``residual + D(act(x @ weight.T + bias))`` in one pass over the product.
+
+    x [..., K], weight [N, K], bias [N] or None, residual [..., N] or None -> [..., N].  ``activation``: "none",
+    "relu", "gelu" (with erf), "gelu_tanh" or "silu".  ``dropout_p``, ``seed``, ``offset``: see the module's text.
+    Gradients flow to x, weight, bias and residual.  With an activation the backward needs x W^T + bias, which the
+    forward then stores in the tensors' type (only where a gradient is wanted); d act(x W^T + bias) is rounded to that
+    type too before the two products of the backward."""
+    _check("linear", x, (("weight", weight), ("bias", bias), ("residual", residual)))
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise RuntimeError(f"linear: weight {list(weight.shape)} does not fit x {list(x.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise RuntimeError(f"linear: bias {list(bias.shape)} does not fit weight {list(weight.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
+        raise RuntimeError(f"linear: residual {list(residual.shape)} is not of the output's shape")
+    if activation not in _lib.DENSE_ACTIVATIONS:
+        raise ValueError(f"linear: activation has to be one of {sorted(_lib.DENSE_ACTIVATIONS)}, got {activation!r}")
+    threshold = _threshold("linear", dropout_p, seed, offset, x.device)
+    code = _lib.DENSE_ACTIVATIONS[activation]
+    if _wants_grad(x, weight, bias, residual):
+        return _Linear.apply(x, weight, bias, residual, code, threshold, seed, offset)
+    return _linear_forward(x, weight, bias, residual, code, threshold, seed, offset, False)[0]
+
+
+# ------------------------------------------------------------------------------------------------
+# residual_norm
+# ------------------------------------------------------------------------------------------------
+def _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop):
+    x, block, weight, bias, post_weight, post_bias, gate = tensors
+    return _lib.DenseNorm(_TYPES[x.dtype], kind, rows, x.shape[-1], gate_rows, eps, scale, x.data_ptr(),
+                          block.data_ptr(), _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
+                          ctypes.pointer(drop) if drop is not None else None)
+
+
+def _norm_forward(tensors, kind, gate_rows, eps, scale, threshold, seed, offset, want_stream, want_stats):
+    lib = _lib.load()
+    tensors = [_contiguous(t) for t in tensors]
+    x = tensors[0]
+    rows = x.numel() // x.shape[-1]
+    y = torch.empty_like(x)
+    stream = torch.empty_like(x) if want_stream else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
+    args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, _drop_struct(threshold, seed, offset))
+    _run("residual_norm", lib.opus_dense_norm_forward, x.device, args, y.data_ptr(), _ptr(stream), _ptr(stats))
+    return y, stream, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, block, weight, bias, post_weight, post_bias, gate, kind, gate_rows, eps, scale, threshold, seed,
+                offset, want_stream):
+        tensors = (x, block, weight, bias, post_weight, post_bias, gate)
+        y, stream, stats = _norm_forward(tensors, kind, gate_rows, eps, scale, threshold, seed, offset, want_stream,
+                                         True)
+        seed_tensor = seed if isinstance(seed, torch.Tensor) and threshold else None
+        ctx.save_for_backward(*tensors, stats, seed_tensor)
+        ctx.settings = kind, gate_rows, eps, scale, threshold, None if seed_tensor is not None else seed, offset
+        ctx.set_materialize_grads(False)
+        return (y, stream) if want_stream else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstream=None):
+        *tensors, stats, seed_tensor = ctx.saved_tensors
+        kind, gate_rows, eps, scale, threshold, seed, offset = ctx.settings
+        none = (None,) * 8
+        if dy is None and dstream is None:
+            return (None,) * 7 + none
+        lib = _lib.load()
+        grads = [torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and need else None
+                 for t, need in zip(tensors, ctx.needs_input_grad)]
+        tensors = [_contiguous(t) for t in tensors]
+        x = tensors[0]
+        rows, width = x.numel() // x.shape[-1], x.shape[-1]
+        dy, dstream = _contiguous(dy), _contiguous(dstream)
+        drop = _drop_struct(threshold, seed if seed_tensor is None else seed_tensor, offset)
+        args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop)
+        need = lib.opus_dense_norm_backward_workspace_bytes(args.type, rows, width,
+                                                            gate_rows if tensors[6] is not None else 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        _run("residual_norm backward", lib.opus_dense_norm_backward, x.device, args, _ptr(dy), _ptr(dstream),
+             stats.data_ptr(), _lib.DenseNormGrads(*[_ptr(g) for g in grads]), _ptr(ws), need)
+        return (*grads, *none)
+
+
+def _gate_rows(x, gate):
+    """How many rows the gate has; row i of x uses gate row i // (rows of x // rows of the gate)."""
+    width, lead = x.shape[-1], x.shape[:-1]
+    if gate.dim() >= 1 and gate.shape[-1] == width:
+        g = gate.shape[:-1]
+        if len(g) == 0 or g == lead:
+            return g.numel()
+        if len(g) == 1 and len(lead) > 0 and g[0] == lead[0]:
+            return g[0]
+        if len(g) == len(lead):
+            n = len(g)
+            while n and g[n - 1] == 1:
+                n -= 1
+            if g[:n] == lead[:n]:
+                return g[:n].numel()
+    raise RuntimeError(f"residual_norm: gate {list(gate.shape)} does not fit x {list(x.shape)}: expected "
+                       f"[{width}], [{lead[0] if len(lead) else 1}, {width}], x's shape, or x's shape with ones for "
+                       f"trailing leading dimensions")
+
+
+def residual_norm(x, block, weight=None, bias=None, kind="layer", eps=1e-5, post_weight=None, post_bias=None, gate=None,
+                  residual_scale=1.0, dropout_p=0.0, seed=None, offset=0, return_stream=False):
+    """The norm between two blocks, with what joins the first block's output to the stream.
+
+        r = residual_scale * x + gate * D(post(block));  y = norm(r)
+
+    x and block [..., width], width at most 16384.  ``kind``: "layer" (mean and variance) or "rms" (mean square), for
+    both norms; ``eps`` is added to the variance (mean square).  weight, bias [width] or None (1 and 0).
+    ``post_weight`` [width] puts a norm of the block's output before the sum (``post_bias`` [width] or None); None:
+    the block's output enters as it is.  ``gate``: [width], one row for each index of x's first dimension
+    ([x.shape[0], width]), one for each row (x's shape), or x's shape with ones in place of its last leading
+    dimensions; None: 1.  ``residual_scale`` is a number.  ``dropout_p``, ``seed``, ``offset``: see the module's text.
+
+    Returns y, or (y, r) with ``return_stream``.  y is computed from the unrounded r.  Gradients flow to all tensors,
+    from either result; the backward computes r again from x and block, so that only two statistics for each norm
+    and row are kept."""
+    _check("residual_norm", x, (("block", block), ("weight", weight), ("bias", bias), ("post_weight", post_weight),
+                                ("post_bias", post_bias), ("gate", gate)))
+    width = x.shape[-1]
+    if block.shape != x.shape:
+        raise RuntimeError(f"residual_norm: block {list(block.shape)} is not of x's shape {list(x.shape)}")
+    if not 1 <= width <= _lib.DENSE_MAX_WIDTH:
+        raise RuntimeError(f"residual_norm: width has to be in [1, {_lib.DENSE_MAX_WIDTH}], got {width}")
+    for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
+        if t is not None and t.shape != (width,):
+            raise RuntimeError(f"residual_norm: {name} {list(t.shape)} has to be [{width}]")
+    if post_bias is not None and post_weight is None:
+        raise RuntimeError("residual_norm: post_bias without post_weight")
+    if kind not in _lib.DENSE_NORMS:
+        raise ValueError(f"residual_norm: kind has to be one of {sorted(_lib.DENSE_NORMS)}, got {kind!r}")
+    gate_rows = 0 if gate is None else _gate_rows(x, gate)
+    threshold = _threshold("residual_norm", dropout_p, seed, offset, x.device)
+    tensors = (x, block, weight, bias, post_weight, post_bias, gate)
+    code = _lib.DENSE_NORMS[kind]
+    if _wants_grad(*tensors):
+        return _ResidualNorm.apply(*tensors, code, gate_rows, eps, residual_scale, threshold, seed, offset,
+                                   return_stream)
+    y, stream, _ = _norm_forward(tensors, code, gate_rows, eps, residual_scale, threshold, seed, offset, return_stream,
+                                 False)
+    return (y, stream) if return_stream else y
+
+
+# ------------------------------------------------------------------------------------------------
+# dropout
+# ------------------------------------------------------------------------------------------------
+def _dropout(x, residual, threshold, seed, offset):
+    lib = _lib.load()
+    x, residual = _contiguous(x), _contiguous(residual)
+    cols = x.shape[-1]
+    y = torch.empty_like(x)
+    _run("dropout", lib.opus_dense_dropout, x.device, _TYPES[x.dtype], x.data_ptr(), _ptr(residual),
+         x.numel() // max(cols, 1), cols, _drop_struct(threshold, seed, offset), y.data_ptr())
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, threshold, seed, offset):
+        seed_tensor = seed if isinstance(seed, torch.Tensor) and threshold else None
+        ctx.save_for_backward(seed_tensor)
+        ctx.settings = threshold, None if seed_tensor is not None else seed, offset
+        return _dropout(x, residual, threshold, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        seed_tensor, = ctx.saved_tensors
+        threshold, seed, offset = ctx.settings
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _dropout(dy, None, threshold, seed if seed_tensor is None else seed_tensor, offset)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x, p, seed, offset=0, residual=None):
+    """``residual + D(x)``: x [..., columns], residual of x's shape or None.  See the module's text for ``D``.
+    Gradients flow to x and residual."""
+    _check("dropout", x, (("residual", residual),))
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"dropout: residual {list(residual.shape)} is not of x's shape {list(x.shape)}")
+    threshold = _threshold("dropout", p, seed, offset, x.device)
+    if _wants_grad(x, residual):
+        return _Dropout.apply(x, residual, threshold, seed, offset)
+    return _dropout(x, residual, threshold, seed, offset)

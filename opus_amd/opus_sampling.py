@@ -23,6 +23,7 @@ import torch
 
 from . import _lib
 from .csrc.wrapper import msmv_sampling, msmv_sampling_rows
+from .opus_dense import linear
 
 
 def relayout_features_torch(mlvl_feats, num_frames, num_views, num_groups):
@@ -273,7 +274,7 @@ def sampling_4d(sample_points, mlvl_feats, scale_weights, occ2img, image_h, imag
 
 
 def sampling_inputs(query_points, query_feat, offset_weight, offset_bias, scale_weight, scale_bias,
-                    num_frames, num_groups, num_points, num_levels, pc_range):
+                    num_frames, num_groups, num_points, num_levels, pc_range, fused=False):
     """What the decoder's sampling module feeds ``sampling_4d`` (restates
     models/opus_transformer.py:337-358 and models/bbox/utils.py:88-93; not pinned by a fixture:
     the module itself needs mmcv to import).
@@ -282,6 +283,7 @@ def sampling_inputs(query_points, query_feat, offset_weight, offset_bias, scale_
     offset_* / scale_* are the weights of the two Linear layers (E -> G*P*3 and E -> G*P*L).
     Returns sample_points [B, Q, T, G, P, 3] (metres, the same points for every frame: an
     expanded view) and scale_weights [B, Q, G, T, P, L] (softmax over levels, expanded over T).
+    ``fused=True`` (GPU tensors) makes the two products with ``opus_dense.linear`` instead of torch's.
     """
     B, Q = query_points.shape[:2]
     T, G, P, L = num_frames, num_groups, num_points, num_levels
@@ -293,8 +295,9 @@ def sampling_inputs(query_points, query_feat, offset_weight, offset_bias, scale_
     else:
         center = pts.mean(dim=2, keepdim=True)
         scale = pts.std(dim=2, keepdim=True)
-    offset = torch.nn.functional.linear(query_feat, offset_weight, offset_bias).view(B, Q, -1, 3)
+    product = linear if fused else torch.nn.functional.linear
+    offset = product(query_feat, offset_weight, offset_bias).view(B, Q, -1, 3)
     sp = (center + offset * scale).view(B, Q, 1, G, P, 3).expand(B, Q, T, G, P, 3)
-    sw = torch.nn.functional.linear(query_feat, scale_weight, scale_bias).view(B, Q, G, 1, P, L)
+    sw = product(query_feat, scale_weight, scale_bias).view(B, Q, G, 1, P, L)
     sw = torch.softmax(sw, dim=-1).expand(B, Q, G, T, P, L)
     return sp, sw

@@ -1,0 +1,657 @@
+"""The dense operators on the GPU against oracle/dense_oracle.py (numpy, 64 bits).
+
+Tolerances are bounds, element by element, from the arithmetic: U[t] = eps / 2 of the output's type for its one
+rounding (plus half the smallest subnormal), and 2^-23 a step of an fp32 sum (a rounding of 2^-24, and as much again
+for what a matrix instruction may drop inside) times the sum of the terms' magnitudes."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import dense_oracle as do
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+U = {t: torch.finfo(t).eps / 2 for t in TYPES.values()}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+STEP = 2.0 ** -23
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+
+
+@pytest.fixture(scope="module")
+def od():
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    from opus_amd import opus_dense
+    return opus_dense
+
+
+def make(rng, dtype, *shape, mean=0.0, std=1.0):
+    return torch.from_numpy(rng.standard_normal(shape) * std + mean).to(dtype).cuda()
+
+
+def f64(t):
+    return None if t is None else t.detach().cpu().double().numpy()
+
+
+def check(got, want, bound, what):
+    got = f64(got)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert np.isfinite(got).all(), f"{what}: non-finite values"
+    over = np.abs(got - want) - bound
+    assert (over <= 0).all(), f"{what}: off by {np.abs(got - want).flat[over.argmax()]:.3e} where {bound.flat[over.argmax()]:.3e} is allowed"
+
+
+def rounded(want, dtype):
+    """what rounding `want` once to dtype may cost"""
+    return U[dtype] * np.abs(want) + TINY[dtype]
+
+
+# ------------------------------------------------------------------------------------------------
+# linear
+# ------------------------------------------------------------------------------------------------
+def linear_bounds(x, w, b, r, dy, name, kept, dtype):
+    """(y, z, bounds of y, dx, dw, db): ez is z's error before any rounding; the backward sees z rounded to dtype
+    (slope'' of the smooth activations is at most 0.8) and rounds dz to it."""
+    K, (M, N) = x.shape[1], (x.shape[0], w.shape[0])
+    y, z = do.linear(x, w, b, name, r, kept)
+    ez = (K + 2) * STEP * (np.abs(x) @ np.abs(w).T + (0 if b is None else np.abs(b)))
+    value, slope = do.act(z, name)
+    # the activation's own arithmetic: a few ulps of value and argument
+    ey = kept * (1.2 * ez + 16 * STEP * (np.abs(value) + np.abs(z) * (name != "none")))
+    by = ey * (1 + U[dtype]) + 2 * STEP * (np.abs(y) + np.abs(0 if r is None else r)) + rounded(y, dtype)
+    if dy is None:
+        return y, by
+    _, _, _, dz = do.linear_backward(dy, x, w, z, name, kept)
+    if name == "none":
+        eslope = np.zeros_like(z)
+    elif name == "relu":
+        eslope = (np.abs(z) <= ez).astype(float)                 # the sign is open there
+    else:
+        eslope = 0.8 * (U[dtype] * np.abs(z) + TINY[dtype] + ez) + 32 * STEP * (1 + np.abs(z))
+    edz = np.abs(dy) * kept * (eslope + 4 * STEP)
+    if name != "none" or not np.isscalar(kept):
+        edz = edz + rounded(np.abs(dz) + edz, dtype)
+    dx, dw, db, _ = do.linear_backward(dy, x, w, z, name, kept)
+    a = np.abs(dz) + edz
+    bx = edz @ np.abs(w) + (N + 2) * STEP * (a @ np.abs(w))
+    bw = edz.T @ np.abs(x) + (M + 2) * STEP * (a.T @ np.abs(x))
+    bb = edz.sum(0) + (M + 2) * STEP * a.sum(0)
+    return y, by, (dx, bx + rounded(dx, dtype) + bx * U[dtype]), (dw, bw + rounded(dw, dtype) + bw * U[dtype]), \
+        (db, bb + rounded(db, dtype) + bb * U[dtype])
+
+
+def run_linear(od, seed, dtype, M, K, N, name="none", bias=True, residual=True, p=0.0, train=True, leave=()):
+    rng = np.random.default_rng(seed)
+    x, w = make(rng, dtype, M, K), make(rng, dtype, N, K, std=max(K, 1) ** -0.5)
+    b = make(rng, dtype, N) if bias else None
+    r = make(rng, dtype, M, N) if residual else None
+    dy = make(rng, dtype, M, N) if train else None
+    kept = do.keep(M, N, p, 77, 5) if p else 1.0
+    inputs = [("x", x), ("w", w), ("b", b), ("r", r)]
+    if train:
+        for n, t in inputs:
+            if t is not None and n not in leave:
+                t.requires_grad_(True)
+    y = od.linear(x, w, b, activation=name, residual=r, dropout_p=p, seed=77, offset=5)
+    assert y.dtype == dtype and y.shape == (M, N)
+    want = linear_bounds(f64(x), f64(w), f64(b), f64(r), f64(dy), name, kept, dtype)
+    what = f"{dtype} M{M} K{K} N{N} {name} p{p}"
+    check(y, want[0], want[1], what + " y")
+    if train:
+        leaves = [(n, t) for n, t in inputs if t is not None and t.requires_grad]
+        grads = dict(zip([n for n, _ in leaves], torch.autograd.grad(y, [t for _, t in leaves], dy)))
+        for n, (g, bound) in zip("xwb", want[2:]):
+            if n in grads:
+                assert grads[n].dtype == dtype
+                check(grads[n], g, bound, f"{what} d{n}")
+        if "r" in grads:
+            assert torch.equal(grads["r"], dy)
+
+
+SIZES = [(1, 8, 8), (1, 1, 1), (3, 1, 5), (1, 1024, 96), (2, 333, 40), (16, 256, 72), (17, 64, 64), (33, 96, 50),
+         (5, 33, 7), (64, 128, 48), (65, 256, 130), (130, 96, 257), (200, 520, 72), (257, 129, 333), (600, 256, 48),
+         (40, 4096, 64), (300, 1000, 520), (129, 2050, 31)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("i", range(len(SIZES)), ids=["x".join(map(str, s)) for s in SIZES])
+def test_linear(od, dtype, i):
+    M, K, N = SIZES[i]
+    run_linear(od, i, TYPES[dtype], M, K, N, name=ACTS[i % 5], bias=i % 3 != 1, residual=i % 2 == 0, p=0.0 if i % 4 else 0.3)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("name", ACTS)
+def test_linear_activations_with_dropout(od, dtype, name):
+    run_linear(od, 50, TYPES[dtype], 70, 72, 88, name=name, p=0.25)
+    run_linear(od, 51, TYPES[dtype], 3, 40, 264, name=name, p=0.0, train=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_linear_many_tiles(od, dtype):
+    """Whole and partial tiles of the wide variants, more than one band of tile rows, all three products."""
+    run_linear(od, 60, TYPES[dtype], 1100, 192, 1300, bias=True, residual=False)
+    run_linear(od, 61, TYPES[dtype], 2049, 136, 776, name="silu", p=0.1)
+    run_linear(od, 62, TYPES[dtype], 1031, 131, 1029, name="gelu")
+
+
+@pytest.mark.parametrize("leave", ["x", "w", "b", "xw", "xb", "wb", "xwr"])
+def test_linear_gradients_asked_for_one_by_one(od, leave):
+    run_linear(od, 70, torch.bfloat16, 150, 136, 72, name="silu", leave=tuple(leave))
+    run_linear(od, 71, torch.float32, 150, 136, 72, leave=tuple(leave))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_linear_sizes_of_zero(od, dtype):
+    for M, K, N in ((0, 16, 8), (4, 0, 8), (4, 16, 0), (0, 0, 0)):
+        run_linear(od, 80, TYPES[dtype], M, K, N)
+        run_linear(od, 81, TYPES[dtype], M, K, N, name="gelu", p=0.5)
+
+
+def test_linear_orders_strides_and_addresses(od):
+    rng = np.random.default_rng(90)
+    for dtype in TYPES.values():
+        buf = make(rng, dtype, 4000)
+        for shift in (0, 1, 3):
+            x = buf[shift:shift + 30 * 40].view(5, 6, 40)
+            w = make(rng, dtype, 40, 24, std=0.1).t()                   # [24, 40], columns first
+            b = make(rng, dtype, 48)[::2]
+            r = make(rng, dtype, 6, 5, 24).transpose(0, 1)
+            y = od.linear(x, w, b, residual=r, activation="silu")
+            want, bound = linear_bounds(f64(x).reshape(30, 40), f64(w), f64(b), f64(r).reshape(30, 24), None, "silu", 1.0, dtype)
+            assert y.is_contiguous()
+            check(y.view(30, 24), want, bound, f"{dtype} shift {shift}")
+        xe = make(rng, dtype, 1, 40).expand(9, 40).detach().requires_grad_(True)
+        y = od.linear(xe, w)
+        g, = torch.autograd.grad(y, xe, torch.ones((), device="cuda", dtype=dtype).expand(9, 24))
+        want, bound = linear_bounds(f64(xe), f64(w), None, None, np.ones((9, 24)), "none", 1.0, dtype)[2]
+        check(g, want, bound, "expanded")
+
+
+def test_linear_non_finite_rows_stay_in_their_rows(od):
+    rng = np.random.default_rng(91)
+    for dtype in TYPES.values():
+        for M, K, N in ((3, 64, 40), (40, 100, 70), (300, 192, 260)):
+            x, w = make(rng, dtype, M, K), make(rng, dtype, N, K)
+            clean = od.linear(x, w)
+            x[1, 5], x[M - 1, K - 1] = float("inf"), float("nan")
+            y = od.linear(x, w)
+            keep = torch.ones(M, dtype=torch.bool)
+            keep[[1, M - 1]] = False
+            assert torch.equal(y[keep], clean[keep])
+            assert not torch.isfinite(y[1]).any() and torch.isnan(y[M - 1]).all()
+            z = w[:, 5].float() != 0
+            assert (torch.isinf(y[1]) == z).all()                       # inf * w, no NaN made of it
+
+
+def test_linear_repeats_bit_for_bit_and_in_place_residual(od):
+    rng = np.random.default_rng(92)
+    x, w, r = (make(rng, torch.float32, *s) for s in ((200, 4096), (64, 4096), (200, 64)))
+    a = od.linear(x, w, residual=r, activation="gelu")
+    for _ in range(3):
+        assert torch.equal(a, od.linear(x, w, residual=r, activation="gelu"))
+
+
+# ------------------------------------------------------------------------------------------------
+# residual_norm
+# ------------------------------------------------------------------------------------------------
+def run_norm(od, seed, dtype, B, T, D, kind="layer", post=True, gate="sample", affine=True, p=0.0, scale=1.0, train=True,
+             want_stream=True, what="", x_scale=1.0):
+    rng = np.random.default_rng(seed)
+    t = {"x": make(rng, dtype, B, T, D, std=x_scale), "block": make(rng, dtype, B, T, D, mean=0.2, std=1.5 * x_scale)}
+    if affine:
+        t["weight"], t["bias"] = make(rng, dtype, D, mean=1, std=0.2), make(rng, dtype, D)
+    if post:
+        t["post_weight"] = make(rng, dtype, D, mean=1, std=0.2)
+        if affine:
+            t["post_bias"] = make(rng, dtype, D)
+    shape = {"none": None, "channel": (D,), "sample": (B, D), "ones": (B, 1, D), "token": (B, T, D)}[gate]
+    if shape:
+        t["gate"] = make(rng, dtype, *shape, mean=0.5)
+    dy, ds = make(rng, dtype, B, T, D), make(rng, dtype, B, T, D)
+    M = B * T
+    if train:
+        for v in t.values():
+            v.requires_grad_(True)
+    kept = do.keep(M, D, p, 31, 2) if p else 1.0
+    res = od.residual_norm(**t, kind=kind, residual_scale=scale, dropout_p=p, seed=31, offset=2, return_stream=want_stream)
+    y, stream = res if want_stream else (res, None)
+
+    a = {n: f64(v) for n, v in t.items()}
+    a["x"], a["block"] = a["x"].reshape(M, D), a["block"].reshape(M, D)
+    if shape:
+        a["gate"] = np.broadcast_to(a["gate"].reshape(B, 1, D) if gate == "sample" else a["gate"], (B, T, D)).reshape(M, D)
+    n64 = dict(dy=f64(dy).reshape(M, D), dstream=f64(ds).reshape(M, D) if want_stream else None) if train else {}
+    want = do.residual_norm(**a, kind=kind, scale=scale, kept=kept, **n64)
+
+    # A row sum in fp32 takes at most 16 + 6 + 16 steps in sequence (a thread's values, the lanes, the waves); a
+    # statistic is off by that, relative to the terms' magnitudes, and enters every element of its row.  C counts those
+    # steps, the few operations around them and the chain of up to four such sums (post mean, post variance, mean,
+    # variance); `size` is the largest magnitude an element's terms have in the row.
+    C = 8 * 40 * STEP
+    one = lambda v, d: np.full(D, d) if v is None else v                        # noqa: E731
+    u_size = np.abs(a["block"])
+    if post:
+        h = a["block"]
+        rs = 1 / np.sqrt((h.var(-1) if kind == "layer" else (h * h).mean(-1)) + 1e-5)[:, None]
+        u_size = (rs * np.abs(h).max(-1, keepdims=True)) * np.abs(one(a.get("post_weight"), 1.0)) + np.abs(one(a.get("post_bias"), 0.0))
+    g = np.abs(a["gate"]) if shape else 1.0
+    r_size = abs(scale) * np.abs(a["x"]) + g * kept * u_size
+    er = C * r_size.max(-1, keepdims=True)
+    r = want["stream"]
+    rstd = 1 / np.sqrt((r.var(-1) if kind == "layer" else (r * r).mean(-1)) + 1e-5)[:, None]
+    hat = (want["y"] - one(a.get("bias"), 0.0)) / one(a.get("weight"), 1.0)
+    w = np.abs(one(a.get("weight"), 1.0))
+    hat_max = np.abs(hat).max(-1, keepdims=True)
+    ehat = rstd * er * (1 + hat_max) + C * hat_max                              # r's own error, and rstd's
+    ey = w * ehat + 4 * STEP * np.abs(one(a.get("bias"), 0.0))
+    what = f"{what}{dtype} {B}x{T}x{D} {kind} post{post} gate {gate} p{p}"
+    check(y.reshape(M, D), want["y"], ey + rounded(want["y"], dtype), what + " y")
+    if want_stream:
+        check(stream.reshape(M, D), r, er + rounded(r, dtype), what + " stream")
+    if not train:
+        return
+    outs, grads = ([y, stream], [dy, ds]) if want_stream else ([y], [dy])
+    got = dict(zip(t, torch.autograd.grad(outs, list(t.values()), grads)))
+
+    def back_error(gin, egin, hat, ehat, rstd):
+        """error of rstd (g - mean g - hat mean(g hat)) for a g off by egin and a hat off by ehat"""
+        gm, hm = np.abs(gin).max(-1, keepdims=True), np.abs(hat).max(-1, keepdims=True)
+        eg, eh = np.max(egin, -1, keepdims=True) + 0 * gm, np.max(ehat, -1, keepdims=True) + 0 * gm
+        dot = np.abs(gin * hat).mean(-1, keepdims=True)
+        edot = eg * np.abs(hat).mean(-1, keepdims=True) + eh * np.abs(gin).mean(-1, keepdims=True) + C * dot
+        return rstd * (2 * eg + C * gm + eh * dot + hm * edot) + (C + ehat / np.maximum(hm, 1)) * rstd * (2 * gm + hm * dot)
+
+    n64dy = f64(dy).reshape(M, D)
+    edr = back_error(n64dy * w, 2 * STEP * np.abs(n64dy) * w, hat, ehat, rstd)
+    ds_size = np.abs(f64(ds).reshape(M, D)) if want_stream else 0.0
+    dr = want["dx"] / scale
+    edr = edr + 4 * STEP * (np.abs(dr) + ds_size)
+    bounds = {"x": abs(scale) * edr}
+    du, edu = dr * (a["gate"] if shape else 1.0) * kept, edr * g * kept
+    edu = edu + 4 * STEP * np.abs(du)
+    u = want["dgate"] / np.where(dr == 0, 1, dr)
+    if post:
+        pw = np.abs(a["post_weight"])
+        hhat = (a["block"] - (a["block"].mean(-1, keepdims=True) if kind == "layer" else 0)) * rs
+        ehh = C * (1 + np.abs(hhat).max(-1, keepdims=True)) ** 2 * (1 + rs * np.abs(a["block"]).max(-1, keepdims=True))
+        bounds["block"] = back_error(du * a["post_weight"], edu * pw, hhat, ehh, rs)
+        eu = kept * (pw * ehh + C * u_size)
+    else:
+        bounds["block"] = edu
+        eu = kept * C * u_size
+    steps = (min(M, 4096) + 64) * STEP
+    total = lambda v, e: e.sum(0) + steps * (np.abs(v) + e).sum(0)              # noqa: E731
+    if affine:
+        bounds["weight"], bounds["bias"] = total(n64dy * hat, np.abs(n64dy) * ehat), total(n64dy, 0 * n64dy)
+    if post:
+        bounds["post_weight"] = total(du * hhat, edu * np.abs(hhat) + np.abs(du) * ehh)
+        if affine:
+            bounds["post_bias"] = total(du, edu)
+    if shape:
+        dg, eg = want["dgate"], edr * np.abs(u) + np.abs(dr) * eu + edr * eu
+        eg = eg + 4 * STEP * np.abs(dg)
+        if gate == "token":
+            bounds["gate"] = eg
+        else:
+            axes = (0, 1) if gate == "channel" else (1,)
+            fold = lambda v: v.reshape(B, T, D).sum(axes)                       # noqa: E731
+            bounds["gate"] = fold(eg) + steps * fold(np.abs(dg) + eg)
+            want["dgate"] = fold(dg)
+    for n in t:
+        ref = want["d" + n]
+        bound = np.broadcast_to(bounds[n], ref.shape) if n in ("x", "block") else bounds[n].reshape(ref.shape)
+        check(got[n].reshape(ref.shape), ref, bound + rounded(ref, dtype), f"{what} d{n}")
+
+
+WIDTHS = [1, 3, 8, 64, 100, 255, 256, 257, 512, 777, 1024, 1025, 2048, 2500, 4096, 5003, 8192, 10001, 16384]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("i", range(len(WIDTHS)), ids=[str(w) for w in WIDTHS])
+def test_norm_widths(od, dtype, i):
+    run_norm(od, i, TYPES[dtype], 2, 3, WIDTHS[i], kind="layer" if i % 2 else "rms", post=i % 3 != 0,
+             gate=["sample", "none", "token", "channel", "ones"][i % 5], p=0.25 if i % 4 == 1 else 0.0, scale=0.5 + 0.25 * (i % 3))
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "sample", "ones", "token"])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("post", [False, True])
+def test_norm_gates(od, gate, kind, post):
+    """Gate rows of many, a few and one row each; whole gate rows by a workgroup, and several workgroups a gate row."""
+    run_norm(od, 40, torch.float32, 5, 61, 72, kind=kind, post=post, gate=gate, p=0.1)
+    run_norm(od, 41, torch.bfloat16, 700, 3, 40, kind=kind, post=post, gate=gate)
+    run_norm(od, 42, torch.float16, 1, 1, 264, kind=kind, post=post, gate=gate, p=0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_norm_many_rows(od, dtype):
+    run_norm(od, 43, TYPES[dtype], 3, 1501, 48, gate="sample", p=0.1)
+    run_norm(od, 44, TYPES[dtype], 2, 1400, 264, kind="rms", gate="channel")
+    run_norm(od, 45, TYPES[dtype], 1, 700, 2056, kind="layer", post=False, gate="none")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_norm_without_affine_gradients_or_stream(od, dtype):
+    run_norm(od, 46, TYPES[dtype], 2, 9, 136, affine=False)
+    run_norm(od, 47, TYPES[dtype], 2, 9, 136, want_stream=False, p=0.3)
+    run_norm(od, 48, TYPES[dtype], 2, 9, 136, train=False, p=0.3)
+    run_norm(od, 49, TYPES[dtype], 1, 1, 4096, kind="rms", train=False, want_stream=False)
+
+
+def test_norm_large_offsets_and_constant_rows(od):
+    """The variance is of deviations from the mean: an offset of 10^4 costs what it must, a constant row gives its bias."""
+    x = torch.full((3, 300), 1e4, device="cuda") + torch.randn(3, 300, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    z = torch.zeros_like(x)
+    y = od.residual_norm(x, z)
+    want = do.residual_norm(f64(x), f64(z))["y"]
+    # an element of 10^4 is off by 0 here (it is the input); its mean by 40 steps
+    assert np.abs(f64(y) - want).max() < 40 * STEP * 1e4 * 2
+    b = torch.randn(300, device="cuda")
+    assert torch.equal(od.residual_norm(torch.full_like(x, 3.0), z, None, b), b.expand(3, 300))
+    assert torch.equal(od.residual_norm(z, z, None, b, kind="rms"), b.expand(3, 300))
+
+
+def test_norm_gradients_asked_for_one_by_one_and_one_result_used(od):
+    rng = np.random.default_rng(5)
+    names = ["x", "block", "weight", "bias", "post_weight", "post_bias", "gate"]
+    shapes = [(6, 11, 72), (6, 11, 72), (72,), (72,), (72,), (72,), (6, 72)]
+    vals = [make(rng, torch.float32, *s) for s in shapes]
+    dy = make(rng, torch.float32, 6, 11, 72)
+
+    def grads(only, which):
+        t = dict(zip(names, [v.clone().requires_grad_(n in only) for n, v in zip(names, vals)]))
+        out = od.residual_norm(**t, return_stream=True)[which]
+        return dict(zip(only, torch.autograd.grad(out, [t[n] for n in only], dy, allow_unused=True)))
+
+    for which in (0, 1):
+        whole = grads(names, which)
+        for n in names:
+            if whole[n] is not None:
+                assert torch.equal(grads([n], which)[n], whole[n]), (which, n)
+    assert grads(names, 1)["weight"] is not None and not grads(names, 1)["weight"].any()
+
+
+def test_norm_no_rows(od):
+    for gate in (None, (0, 16), (16,), (0, 5, 16)):
+        t = {"x": torch.zeros(0, 5, 16, device="cuda"), "block": torch.zeros(0, 5, 16, device="cuda"),
+             "weight": torch.ones(16, device="cuda")}
+        if gate:
+            t["gate"] = torch.ones(gate, device="cuda")
+        for v in t.values():
+            v.requires_grad_(True)
+        y = od.residual_norm(**t)
+        got = dict(zip(t, torch.autograd.grad(y, list(t.values()), torch.zeros_like(y))))
+        assert y.shape == (0, 5, 16) and not got["weight"].any() and all(got[n].shape == t[n].shape for n in t)
+        assert not any(torch.isnan(v).any() for v in got.values())
+    t = {"x": torch.zeros(3, 0, 16, device="cuda", requires_grad=True), "block": torch.zeros(3, 0, 16, device="cuda"),
+         "gate": torch.ones(3, 16, device="cuda", requires_grad=True)}
+    y = od.residual_norm(**t)
+    assert not torch.autograd.grad(y, t["gate"], torch.zeros_like(y))[0].any()
+
+
+# ------------------------------------------------------------------------------------------------
+# dropout
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(1, 1), (7, 1), (1, 8), (5, 3), (33, 20), (100, 256), (3, 4097), (300, 1003), (1, 70001)])
+def test_dropout(od, dtype, rows, cols):
+    dtype = TYPES[dtype]
+    rng = np.random.default_rng(rows + cols)
+    for p, residual in ((0.1, True), (0.5, False), (1.0, True), (0.0, True)):
+        x = make(rng, dtype, rows, cols).requires_grad_(True)
+        r = make(rng, dtype, rows, cols).requires_grad_(True) if residual else None
+        dy = make(rng, dtype, rows, cols)
+        y = od.dropout(x, p, 2 ** 63 + 11, offset=9, residual=r)
+        k = do.keep(rows, cols, p, 2 ** 63 + 11, 9)
+        want = f64(x) * k + (f64(r) if residual else 0.0)
+        check(y, want, rounded(want, dtype) + 4 * STEP * (np.abs(f64(x) * k) + np.abs(want)), f"p {p}")
+        if p == 1.0:
+            assert torch.equal(y, r)
+        g = torch.autograd.grad(y, [x] + ([r] if residual else []), dy)
+        check(g[0], f64(dy) * k, rounded(f64(dy) * k, dtype) + 4 * STEP * np.abs(f64(dy) * k), "dx")
+        if residual:
+            assert torch.equal(g[1], dy)
+
+
+def test_one_mask_whatever_the_operator_type_and_shape(od):
+    rows, cols, p = 70, 100, 0.3
+    k = do.keep(rows, cols, p, 123, 4) != 0
+    eye = torch.eye(cols, device="cuda")
+    for dtype in TYPES.values():
+        one = torch.ones(rows, cols, device="cuda", dtype=dtype)
+        assert np.array_equal(f64(od.dropout(one, p, 123, 4)) != 0, k)
+        assert np.array_equal(f64(od.dropout(one.view(7, 10, cols), p, 123, 4)).reshape(rows, cols) != 0, k)
+        assert np.array_equal(f64(od.linear(one, eye.to(dtype), dropout_p=p, seed=123, offset=4)) != 0, k)
+        stream = od.residual_norm(torch.zeros_like(one), one, dropout_p=p, seed=123, offset=4, return_stream=True)[1]
+        assert np.array_equal(f64(stream) != 0, k)
+    seed = torch.tensor(123, device="cuda")
+    assert np.array_equal(f64(od.dropout(one, p, seed, 4)) != 0, k)
+    assert np.array_equal(f64(od.dropout(one, p, 123 - 2 ** 64, 4)) != 0, k)
+
+
+def test_dropped_values_are_zero_whatever_they_were(od):
+    x = torch.full((64, 64), float("nan"), device="cuda")
+    y = od.dropout(x, 0.5, 1)
+    k = do.keep(64, 64, 0.5, 1) != 0
+    assert np.array_equal(np.isnan(f64(y)), k) and not f64(y)[~k].any()
+
+
+def test_as_many_rows_as_a_launch_takes(od):
+    """2^31 rows of two columns (8 GiB), both ends; 2^32 rows would be more threads than a launch counts: refused."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of device memory")
+    x = torch.ones(2 ** 32, 1, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="too large"):
+        od.dropout(x, 0.5, 3)
+    y = od.dropout(x.view(2 ** 31, 2), 0.5, 3)
+    for first in (0, 2 ** 31 - 64):
+        want = do.keep(64, 2, 0.5, 3, first_row=first)
+        assert np.array_equal(f64(y[first:first + 64]), want)
+
+
+# ------------------------------------------------------------------------------------------------
+# streams, graphs, devices, seeds, refusals
+# ------------------------------------------------------------------------------------------------
+def layer(od, t, seed, offset=0):
+    """What follows the sampling in a decoder layer: way back into the stream, norm, feed-forward block, norm."""
+    h = od.linear(t["sampled"], t["w0"], t["b0"])
+    q = od.residual_norm(t["query"], h, t["g0"], t["h0"], dropout_p=0.1, seed=seed, offset=offset)
+    f = od.linear(q, t["w1"], t["b1"], activation="relu", dropout_p=0.1, seed=seed, offset=offset + 1)
+    s = od.linear(f, t["w2"], t["b2"], dropout_p=0.1, seed=seed, offset=offset + 2, residual=q)
+    return od.residual_norm(torch.zeros_like(s), s, t["g1"], t["h1"])
+
+
+def layer_tensors(dtype=torch.float32, Q=150, E=64, S=512, F=128):
+    gen = torch.Generator("cuda").manual_seed(3)
+    n = lambda *s, std=1.0: (torch.randn(s, generator=gen, device="cuda") * std).to(dtype)        # noqa: E731
+    return {"sampled": n(2, Q, S), "query": n(2, Q, E), "w0": n(E, S, std=S ** -0.5), "b0": n(E), "g0": 1 + n(E, std=0.1),
+            "h0": n(E), "w1": n(F, E, std=E ** -0.5), "b1": n(F), "w2": n(E, F, std=F ** -0.5), "b2": n(E),
+            "g1": 1 + n(E, std=0.1), "h1": n(E)}
+
+
+def test_operators_together_with_the_sampling(od):
+    """A decoder layer's sampling and what follows it, forward and backward, against the same in torch, fp64 on the CPU,
+    from the sampled features on."""
+    from opus_amd import opus_sampling
+    from helpers import sampling4d_case, TINY_LEVELS
+    B, Q, T, G, P, N, E = 1, 60, 2, 4, 2, 6, 256
+    _, _, occ2img = sampling4d_case(5, B, Q, T, G, P, N=N)
+    gen = torch.Generator("cuda").manual_seed(9)
+    n = lambda *s, std=1.0: torch.randn(s, generator=gen, device="cuda") * std                    # noqa: E731
+    feats = [n(B * T * G, N, h, w, 64).requires_grad_(True) for h, w in TINY_LEVELS]
+    query = n(B, Q, E).requires_grad_(True)
+    points = torch.rand((B, Q, 8, 3), generator=gen, device="cuda")
+    ow, ob, sw, sb = n(G * P * 3, E, std=0.06), n(G * P * 3), n(G * P * 4, E, std=0.06), n(G * P * 4)
+    rng = [-40.0, -40.0, -1.0, 40.0, 40.0, 5.4]
+    inputs = (points, query, ow, ob, sw, sb, T, G, P, 4, rng)
+    sp, scales = opus_sampling.sampling_inputs(*inputs, fused=True)
+    sp0, scales0 = opus_sampling.sampling_inputs(*inputs)
+    # two fp32 products of 256 terms of about 1/16 .. apart: 258 steps times the sum of magnitudes, times the points' spread
+    assert (scales - scales0).abs().max() < 4 * 258 * STEP * 256 * 0.06
+    assert (sp - sp0).abs().max() < 4 * 258 * STEP * 256 * 0.06 * 30
+    out = opus_sampling.sampling_4d(sp, feats, scales, torch.from_numpy(occ2img).cuda(), 256, 704, N)
+    t = layer_tensors(E=E, S=G * T * P * 64)
+    t["sampled"], t["query"] = out.reshape(B, Q, -1), query
+    y = layer(od, t, 21)
+    grad = n(B, Q, E)
+    sampled = t["sampled"]
+    got = torch.autograd.grad(y, [sampled, query, *feats], grad)
+    assert all(torch.isfinite(g).all() for g in got) and all(g.abs().max() > 0 for g in got)
+
+    d = {k: v.detach().cpu().double() for k, v in t.items()}
+    d["sampled"].requires_grad_(True)
+    d["query"].requires_grad_(True)
+    F = torch.nn.functional
+    k = [torch.from_numpy(do.keep(B * Q, c, 0.1, 21, i)).view(B, Q, c) for i, c in enumerate((E, 128, E))]
+    q = F.layer_norm(d["query"] + k[0] * F.linear(d["sampled"], d["w0"], d["b0"]), (E,), d["g0"], d["h0"])
+    f = k[1] * F.linear(q, d["w1"], d["b1"]).relu()
+    want = F.layer_norm(q + k[2] * F.linear(f, d["w2"], d["b2"]), (E,), d["g1"], d["h1"])
+    # fp32 end to end: each product's error is at most (terms + 2) steps of sums of magnitudes near sqrt(terms), and the
+    # norms pass it on with a factor near 1: 1026 * 2^-23 * sqrt(1024) bounds it, in practice by far
+    tol = 1026 * STEP * 32
+    assert (y.detach().cpu().double() - want.detach()).abs().max() < tol
+    ws, = torch.autograd.grad(want, d["sampled"], grad.cpu().double())
+    # a relu whose sign the rounding decides would show: compare where all but a few agree
+    off = (got[0].cpu().double() - ws).abs().flatten()
+    assert off.kthvalue(int(off.numel() * 0.99)).values < tol
+
+
+def test_other_streams(od):
+    t = layer_tensors()
+    want = layer(od, t, 4)
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in side:
+        with torch.cuda.stream(s):
+            outs.append(layer(od, t, 4))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_captured_step_replays_with_new_inputs_and_seeds(od, dtype):
+    """Forward and backward in one graph; the seed is a tensor that the graph's user changes between replays."""
+    t = layer_tensors(TYPES[dtype])
+    leaves = [v.requires_grad_(True) for v in t.values()]
+    grad = torch.randn_like(t["query"])
+    seed = torch.tensor([5], device="cuda")
+
+    def step():
+        y = layer(od, t, seed)
+        return [y, *torch.autograd.grad(y, leaves, grad)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        with torch.no_grad():
+            seed.fill_(100 + turn)
+            t["sampled"].normal_()
+        graph.replay()
+        got = [o.detach().clone() for o in out]
+        torch.cuda.synchronize()
+        want = step()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b.detach())
+    seeds = []
+    for turn in range(2):
+        with torch.no_grad():
+            seed.fill_(turn)
+        graph.replay()
+        seeds.append(out[0].detach().clone())
+    assert not torch.equal(*seeds)
+
+
+def test_two_captured_graphs_replayed_in_turn(od):
+    """Graphs that are captured one after the other own their workspaces (the product's r is cut up here)."""
+    rng = np.random.default_rng(6)
+    xs = [make(rng, torch.bfloat16, 64, 4096) for _ in range(2)]
+    w = make(rng, torch.bfloat16, 64, 4096, std=0.02)
+    want = [od.linear(x, w) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(od.linear(x, w))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, want):
+            assert torch.equal(o, e)
+
+
+def test_seed_tensor_changed_before_the_backward_is_an_error(od):
+    seed = torch.tensor([5], device="cuda")
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    y = od.dropout(x, 0.5, seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_gradients_against_differences(od):
+    """Directional derivatives of the GPU operators themselves, fp32, central differences: with a step of 2^-6 along a
+    unit direction the difference's own error is h^2 / 6 of a third derivative (order 1 here) plus rounding of the loss
+    (sum of about 10^3 terms: 2^-24 * 10^3 / h)."""
+    t = layer_tensors(Q=20, E=32, S=64, F=40)
+    gen = torch.Generator("cuda").manual_seed(8)
+    x, w, b = t["sampled"], torch.randn((48, 64), generator=gen, device="cuda") * 0.125, torch.randn(48, generator=gen, device="cuda")
+    c = torch.randn((2, 20, 48), generator=gen, device="cuda")
+    blk, gate = torch.randn((2, 20, 64), generator=gen, device="cuda"), torch.randn((2, 64), generator=gen, device="cuda")
+    c2 = torch.randn((2, 20, 64), generator=gen, device="cuda")
+    f1 = lambda x, w, b: (od.linear(x, w, b, activation="gelu", dropout_p=0.2, seed=3).double() * c).sum()         # noqa: E731
+    f2 = lambda x, blk, gate: (od.residual_norm(x, blk, post_weight=torch.ones(64, device="cuda"), gate=gate,      # noqa: E731
+                                                dropout_p=0.2, seed=3).double() * c2).sum()
+    f3 = lambda x: (od.dropout(x, 0.2, 3).double() ** 2 / 2).sum()                                                 # noqa: E731
+    h = 2.0 ** -6
+    for f, args in ((f1, (x, w, b)), (f2, (x, blk, gate)), (f3, (x,))):
+        args = [a.detach().clone().requires_grad_(True) for a in args]
+        grads = torch.autograd.grad(f(*args), args)
+        for i, a in enumerate(args):
+            v = torch.randn(a.shape, generator=gen, device="cuda")
+            v = v / v.norm()
+            with torch.no_grad():
+                up = f(*[q + h * v if j == i else q for j, q in enumerate(args)])
+                down = f(*[q - h * v if j == i else q for j, q in enumerate(args)])
+            slope = (grads[i].double() * v).sum()
+            assert abs((up - down) / (2 * h) - slope) < 20 * (h * h + 2.0 ** -24 * 1e3 / h) * (1 + abs(slope))
+
+
+def test_refusals(od):
+    x, w = torch.zeros(4, 16, device="cuda"), torch.zeros(8, 16, device="cuda")
+    bad = [lambda: od.linear(x, w.half()), lambda: od.linear(x, w[:, :15]), lambda: od.linear(x, w[0]),
+           lambda: od.linear(x, w, torch.zeros(7, device="cuda")), lambda: od.linear(x, w, torch.zeros(8)),
+           lambda: od.linear(x, w, residual=torch.zeros(4, 7, device="cuda")), lambda: od.linear(x.double(), w.double()),
+           lambda: od.linear(x, w, residual=torch.zeros(1, 8, device="cuda")),
+           lambda: od.linear(x, w, dropout_p=0.5), lambda: od.linear(x, w, dropout_p=0.5, seed=torch.zeros(1, dtype=torch.int64)),
+           lambda: od.linear(torch.zeros((), device="cuda"), w), lambda: od.linear(x, w, activation="tanh"),
+           lambda: od.linear(x, w, dropout_p=1.5, seed=1), lambda: od.linear(x, w, dropout_p=0.5, seed=1, offset=-1),
+           lambda: od.residual_norm(x, x[:2]), lambda: od.residual_norm(x, x, w), lambda: od.residual_norm(x, x, kind="batch"),
+           lambda: od.residual_norm(x, x, post_bias=x[0]), lambda: od.residual_norm(x, x, gate=x[:3]),
+           lambda: od.residual_norm(x, x.half()), lambda: od.residual_norm(x[:, :0], x[:, :0]),
+           lambda: od.residual_norm(torch.zeros(1, 16385, device="cuda"), torch.zeros(1, 16385, device="cuda")),
+           lambda: od.dropout(x, 0.5, None), lambda: od.dropout(x, -0.5, 1), lambda: od.dropout(x, 0.5, 1, residual=x[0]),
+           lambda: od.dropout(x.int(), 0.5, 1)]
+    for i, f in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError)):
+            f()
+            raise AssertionError(f"call {i} was taken")
+
+
+def test_no_second_derivatives(od):
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(od.dropout(x, 0.5, 1).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

@@ -39,14 +39,15 @@ struct Epilogue {
     DnDrop drop;
 };
 
-// v: eight values of C at (row, col ..), `n` of them inside; col is a multiple of 8.
-template <class T>
-__device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, uint64_t row, uint32_t col, int n,
-                                       uint32_t cols, uint64_t seed)
+// v: eight values of C at (row, col ..), element `at` of y, `n` of them inside (all of them, where !EDGE); col is a
+// multiple of 8.  bias: those columns' (zeros without one).
+template <class T, bool EDGE>
+__device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, const dn_floats<8> &bias, uint64_t at, uint64_t row,
+                                       uint32_t col, int n, uint64_t seed)
 {
-    const uint64_t at = row * cols + col;
-    if (e.bias)
-        v += dn_load_n<8>(static_cast<const T *>(e.bias) + col, n);
+    if (!EDGE)
+        n = 8;
+    v += bias;
     if (e.z) {
         dn_floats<8> z = v;
         // fp16: a tiny z must not become 0, or relu's gradient would take it for a negative one
@@ -74,7 +75,8 @@ struct GemmArgs {
     int tiles_i, tiles_j, splits, steps, steps_per_split;       // steps: tiles of 128 bytes along r
     float *partial;              // [splits][I][pitch], where splits > 1
     long long pitch;
-    float *colsum;               // [splits][I]: sum over r of A(i, r), NULL: not wanted
+    float *colsum;               // [splits * sharers][I]: sum over r of A(i, r), NULL: not wanted
+    int sharers;                 // tiles of a row of tiles that share the column sums' work, times the waves side by side
     Epilogue e;
 };
 
@@ -116,55 +118,70 @@ struct Tile {
         }
     }
 
-    // Straight to LDS.  Rows beyond `I` (columns, where !RC) fetch the last valid one: what they make of C is never
-    // stored.  `r0 + STEP <= R`, 16-byte aligned rows.
+    // Straight to LDS: a thread's pieces of the first tile, in bytes from the tile's base; the following tiles are a
+    // uniform distance further.  Rows beyond `I` (columns, where !RC) fetch the last valid one: what they make of C is
+    // never stored.
     template <int THREADS>
-    static __device__ __forceinline__ void fetch(const T *base, long long w0, long long r0, long long I, long long R,
-                                                 char *lds, int wave, int lane)
+    static __device__ __forceinline__ void offsets(uint32_t (&off)[PIECES / THREADS], long long w0, long long I, long long R, int tid)
     {
         static_assert(PIECES % THREADS == 0, "whole turns");
 #pragma unroll
         for (int t = 0; t < PIECES / THREADS; ++t) {
-            const int first = t * THREADS + wave * 64;
             int w, r;
-            coords(first + lane, w, r);
-            const T *src;
-            if constexpr (RC) {
-                const long long row = min(w0 + w, I - 1);
-                src = base + row * R + (r0 + r);
-            } else {
-                const long long col = min(w0 + w, I - PIECE);
-                src = base + (r0 + r) * I + col;
-            }
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                             (__attribute__((address_space(3))) void *)(lds + first * 16), 16, 0, 0);
+            coords(t * THREADS + tid, w, r);
+            if constexpr (RC)
+                off[t] = (uint32_t)(min((long long)w, I - 1 - w0) * R + r) * sizeof(T);
+            else
+                off[t] = (uint32_t)(r * I + min((long long)w, I - PIECE - w0)) * sizeof(T);
         }
+    }
+    // the tile's base, and how far the next one is
+    static __device__ __forceinline__ const char *origin(const T *base, long long w0, long long r0, long long I, long long R)
+    {
+        return reinterpret_cast<const char *>(RC ? base + w0 * R + r0 : base + r0 * I + w0);
+    }
+    static __device__ __forceinline__ long long advance(long long I) { return RC ? STEP * sizeof(T) : STEP * I * sizeof(T); }
+
+    template <int THREADS>
+    static __device__ __forceinline__ void fetch(const char *from, const uint32_t (&off)[PIECES / THREADS], char *lds, int wave)
+    {
+#pragma unroll
+        for (int t = 0; t < PIECES / THREADS; ++t)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + off[t]),
+                                             (__attribute__((address_space(3))) void *)(lds + (t * THREADS + wave * 64) * 16),
+                                             16, 0, 0);
     }
 
     // Through registers: any alignment, zeros outside.
+    template <int THREADS> using Pieces = typename DnVec<T, PIECE>::type[PIECES / THREADS];
+
     template <int THREADS>
-    static __device__ __forceinline__ void copy(const T *base, long long w0, long long r0, long long I, long long R,
-                                                char *lds, int tid)
+    static __device__ __forceinline__ void read(Pieces<THREADS> &v, const T *base, long long w0, long long r0, long long I,
+                                                long long R, int tid)
     {
 #pragma unroll
         for (int t = 0; t < PIECES / THREADS; ++t) {
-            const int p = t * THREADS + tid;
             int w, r;
-            coords(p, w, r);
-            typename DnVec<T, PIECE>::type v = (T)0.f;
+            coords(t * THREADS + tid, w, r);
+            v[t] = (T)0.f;
             const long long i = w0 + w, rr = r0 + r;
             const T *src = RC ? base + i * R + rr : base + rr * I + i;
             const long long inside = RC ? (i < I ? R - rr : 0) : (rr < R ? I - i : 0);
             if (inside >= PIECE) {
-                v = dn_load<PIECE>(src);
+                v[t] = dn_load<PIECE>(src);
             } else {
 #pragma unroll
                 for (int j = 0; j < PIECE; ++j)
                     if (j < inside)
-                        v[j] = src[j];
+                        v[t][j] = src[j];
             }
-            *reinterpret_cast<typename DnVec<T, PIECE>::type *>(lds + p * 16) = v;
         }
+    }
+    template <int THREADS> static __device__ __forceinline__ void write(const Pieces<THREADS> &v, char *lds, int tid)
+    {
+#pragma unroll
+        for (int t = 0; t < PIECES / THREADS; ++t)
+            *reinterpret_cast<typename DnVec<T, PIECE>::type *>(lds + (t * THREADS + tid) * 16) = v[t];
     }
 
     // A lane's operands of rows w .. w+31 (lane % 32) for k-group `ks` (of 4): RC order of r: pieces 2 ks + lane / 32.
@@ -212,6 +229,27 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c)
     return c;
 }
 
+// s + the lane's values of an operand (two at a time: products with one)
+__device__ __forceinline__ float add_up(bf16x8 v, float s)
+{
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int t = 0; t < 8; t += 2)
+        s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[t], v[t + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float add_up(f16x8 v, float s)
+{
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+    for (int t = 0; t < 8; t += 2)
+        s = __builtin_amdgcn_fdot2(f16x2{v[t], v[t + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float add_up(f32x4 v, float s) { return s + ((v[0] + v[1]) + (v[2] + v[3])); }
+
 constexpr int STRIP = 72;       // floats a row of a wave's strip in LDS: rows four apart then start 32 banks apart
 
 // WI x WJ waves, each MI x MJ blocks of 32 x 32.  DIRECT: bases and rows are 16-byte aligned.
@@ -243,15 +281,30 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
     const int s0 = split * g.steps_per_split, s1 = min(s0 + g.steps_per_split, g.steps);
 
     const T *pa = static_cast<const T *>(g.a), *pb = static_cast<const T *>(g.b);
-    const auto stage = [&](int s, char *to) {
-        const long long r0 = (long long)s * STEP;
-        if (DIRECT && r0 + STEP <= g.R) {
-            TA::template fetch<THREADS>(pa, i0, r0, g.I, g.R, to, wave, lane);
-            TB::template fetch<THREADS>(pb, j0, r0, g.J, g.R, to + TA::BYTES, wave, lane);
-        } else {
-            TA::template copy<THREADS>(pa, i0, r0, g.I, g.R, to, tid);
-            TB::template copy<THREADS>(pb, j0, r0, g.J, g.R, to + TA::BYTES, tid);
-        }
+    typename TA::template Pieces<THREADS> va;
+    typename TB::template Pieces<THREADS> vb;
+    const auto read = [&](int s) __attribute__((always_inline)) {
+        TA::template read<THREADS>(va, pa, i0, (long long)s * STEP, g.I, g.R, tid);
+        TB::template read<THREADS>(vb, pb, j0, (long long)s * STEP, g.J, g.R, tid);
+    };
+    const auto write = [&](char *to) __attribute__((always_inline)) {
+        TA::template write<THREADS>(va, to, tid);
+        TB::template write<THREADS>(vb, to + TA::BYTES, tid);
+    };
+    // whole tiles, which may go straight to LDS; the last one of all may not be
+    const int whole = DIRECT ? min(s1, (int)(g.R / STEP)) : s0;
+    uint32_t oa[TA::PIECES / THREADS], ob[TB::PIECES / THREADS];
+    const char *fa0 = TA::origin(pa, i0, (long long)s0 * STEP, g.I, g.R), *fb0 = TB::origin(pb, j0, (long long)s0 * STEP, g.J, g.R);
+    const long long na = TA::advance(g.I), nb = TB::advance(g.J);
+    if constexpr (DIRECT) {
+        TA::template offsets<THREADS>(oa, i0, g.I, g.R, tid);
+        TB::template offsets<THREADS>(ob, j0, g.J, g.R, tid);
+    }
+    const auto fetch = [&](char *to) __attribute__((always_inline)) {
+        TA::template fetch<THREADS>(fa0, oa, to, wave);
+        TB::template fetch<THREADS>(fb0, ob, to + TA::BYTES, wave);
+        fa0 += na;
+        fb0 += nb;
     };
 
     f32x16 acc[MI][MJ];
@@ -264,47 +317,87 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
 #pragma unroll
     for (int i = 0; i < MI; ++i)
         sum[i] = 0.f;
-    const bool want_sum = !ARC && g.colsum && tj == 0 && wj == 0;
+    // The sums of A's rows: of a row of tiles the first `share` take turns at the steps of r, and of the waves that hold
+    // the same rows each takes its k-groups of a step.
+    const int share = g.sharers / WJ;
+    const bool summing = !ARC && g.colsum && tj < share;
 
-    if (s0 < s1)
-        stage(s0, lds);
-    for (int s = s0; s < s1; ++s) {
-        const int buf = (s - s0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (s + 1 < s1)
-            stage(s + 1, lds + (buf ^ 1) * STAGE);
-        const char *la = lds + buf * STAGE, *lb = la + TA::BYTES;
+    typename DnVec<T, Elem<T>::PIECE>::type fa[2][MI], fb[2][MJ];
+    const auto load = [&](const char *from, int ks) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            typename DnVec<T, Elem<T>::PIECE>::type fa[MI], fb[MJ];
+        for (int i = 0; i < MI; ++i)
+            fa[ks & 1][i] = TA::frag(from, (wi * MI + i) * 32, ks, lane);
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
-                fa[i] = TA::frag(la, (wi * MI + i) * 32, ks, lane);
+        for (int j = 0; j < MJ; ++j)
+            fb[ks & 1][j] = TB::frag(from + TA::BYTES, (wj * MJ + j) * 32, ks, lane);
+    };
+    bool turn_to_sum = false;
+    const auto multiply = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < MJ; ++j)
-                fb[j] = TB::frag(lb, (wj * MJ + j) * 32, ks, lane);
+                acc[i][j] = mma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j]);
+        if (!ARC && turn_to_sum && ks % WJ == wj)
 #pragma unroll
             for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < MJ; ++j)
-                    acc[i][j] = mma(fa[i], fb[j], acc[i][j]);
-            if (!ARC && want_sum)
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int t = 0; t < Elem<T>::PIECE; ++t)
-                        sum[i] += (float)fa[i][t];
+                sum[i] = add_up(fa[ks & 1][i], sum[i]);
+    };
+    // One barrier a tile, before its last k-group is multiplied: by then every wave holds that group in registers, so
+    // the tile's buffer is free for the transfers of the tile after next, and the next tile, under way for a whole
+    // tile's time, is complete; its first group is read while the last of this one is multiplied.
+    const auto arrived = [] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    if (s0 < s1) {
+        char *cur = lds, *next = lds + STAGE;
+        if (DIRECT && s0 < whole) {
+            fetch(cur);
+        } else {
+            read(s0);
+            write(cur);
+        }
+        arrived();
+        if (DIRECT && s0 + 1 < whole)
+            fetch(next);
+        load(cur, 0);
+        for (int s = s0; s < s1; ++s) {
+            turn_to_sum = summing && s % share == tj;
+            const bool more = s + 1 < s1, by_hand = more && s + 1 >= whole;
+            if (!DIRECT && by_hand)             // under way while this tile is multiplied
+                read(s + 1);
+            load(cur, 1);
+            multiply(0);
+            load(cur, 2);
+            multiply(1);
+            load(cur, 3);
+            multiply(2);
+            if (more) {
+                if (by_hand) {
+                    if (DIRECT)                 // one tile of a product: not worth the registers it would hold
+                        read(s + 1);
+                    write(next);
+                }
+                arrived();
+                if (DIRECT && s + 2 < whole)
+                    fetch(cur);
+                load(next, 0);
+            }
+            multiply(3);
+            char *t = cur;
+            cur = next;
+            next = t;
         }
     }
 
-    if (!ARC && want_sum)
+    if (!ARC && summing)
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             const float t = sum[i] + __shfl_xor(sum[i], 32);
             const long long row = i0 + (wi * MI + i) * 32 + (lane & 31);
             if (lane < 32 && row < g.I)
-                g.colsum[split * g.I + row] = t;
+                g.colsum[((long long)split * g.sharers + tj * WJ + wj) * g.I + row] = t;
         }
 
     // ---- epilogue: a wave turns 32 rows x (32 MJ, at most 64) columns at a time through its own strip
@@ -312,34 +405,56 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
     const uint64_t seed = dn_seed(g.e.drop);
     float *strip = reinterpret_cast<float *>(lds) + wave * 32 * STRIP;
     __syncthreads();
+    const bool inside = i0 + BM <= g.I && j0 + BN <= g.J;
+    // one turn of the loop a strip: the code behind it exists once, whatever the number of blocks
+#pragma unroll 1
+    for (int turn = 0; turn < MI * MJ / SJ; ++turn) {
+        const int i = turn / (MJ / SJ), jj = turn % (MJ / SJ) * SJ;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int k = 0; k < MI * MJ / SJ; ++k)
+            if (turn == k)
 #pragma unroll
-        for (int jj = 0; jj < MJ; jj += SJ) {
+                for (int j = 0; j < SJ; ++j)
 #pragma unroll
-            for (int j = 0; j < SJ; ++j)
+                    for (int t = 0; t < 16; ++t)
+                        strip[((t >> 2) * 8 + (lane >> 5) * 4 + (t & 3)) * STRIP + j * 32 + (lane & 31)] =
+                            acc[k / (MJ / SJ)][k % (MJ / SJ) * SJ + j][t];
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int col = (lane % CPR) * 8;
+        const float *from = strip + lane / CPR * STRIP + col;
+        const long long ci = i0 + (wi * MI + i) * 32 + lane / CPR, cj = j0 + (wj * MJ + jj) * 32 + col;
+        const auto value = [&](int q) __attribute__((always_inline)) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(from + q * RPT * STRIP);
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(from + q * RPT * STRIP + 4);
+            return (dn_floats<8>)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        if (g.partial) {
+            float *to = g.partial + (split * g.I + ci) * g.pitch + cj;
 #pragma unroll
-                for (int t = 0; t < 16; ++t)
-                    strip[((t >> 2) * 8 + (lane >> 5) * 4 + (t & 3)) * STRIP + j * 32 + (lane & 31)] = acc[i][jj + j][t];
-            __builtin_amdgcn_wave_barrier();
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int q = 0; q < 32 / RPT; ++q)
+                if (ci + q * RPT < g.I && cj < g.J)
+                    *reinterpret_cast<dn_floats<8> *>(to + q * RPT * g.pitch) = value(q);
+        } else {
+            const int n = (int)min(8ll, g.J - cj);
+            dn_floats<8> bias = 0.f;
+            if (g.e.bias)
+                bias = dn_load_n<8>(static_cast<const T *>(g.e.bias) + cj, n);
+            uint64_t at = (uint64_t)ci * g.J + cj;
+            if (inside) {
 #pragma unroll
-            for (int q = 0; q < 32 / RPT; ++q) {
-                const int row = q * RPT + lane / CPR, col = (lane % CPR) * 8;
-                const f32x4 lo = *reinterpret_cast<const f32x4 *>(strip + row * STRIP + col);
-                const f32x4 hi = *reinterpret_cast<const f32x4 *>(strip + row * STRIP + col + 4);
-                const long long ci = i0 + (wi * MI + i) * 32 + row, cj = j0 + (wj * MJ + jj) * 32 + col;
-                const dn_floats<8> v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                if (ci < g.I && cj < g.J) {
-                    if (g.partial)
-                        *reinterpret_cast<dn_floats<8> *>(g.partial + (split * g.I + ci) * g.pitch + cj) = v;
-                    else
-                        finish<T>(g.e, v, ci, (uint32_t)cj, (int)min(8ll, g.J - cj), (uint32_t)g.J, seed);
-                }
+                for (int q = 0; q < 32 / RPT; ++q, at += RPT * g.J)
+                    finish<T, false>(g.e, value(q), bias, at, ci + q * RPT, (uint32_t)cj, 8, seed);
+            } else {
+#pragma unroll 1
+                for (int q = 0; q < 32 / RPT; ++q, at += RPT * g.J)
+                    if (ci + q * RPT < g.I && n > 0)
+                        finish<T, true>(g.e, value(q), bias, at, ci + q * RPT, (uint32_t)cj, n, seed);
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_wave_barrier();
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // Adds the shares of r in order and runs the epilogue; a thread takes eight columns of a row.
@@ -357,20 +472,34 @@ __global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g)
     const float *p = g.partial + row * g.pitch + col;
     for (int s = 0; s < g.splits; ++s, p += g.I * g.pitch)
         v += *reinterpret_cast<const dn_floats<8> *>(p);
-    finish<T>(g.e, v, row, col, (int)min((long long)8, g.J - (long long)col), (uint32_t)g.J, seed);
+    const int n = (int)min(8ll, g.J - (long long)col);
+    dn_floats<8> bias = 0.f;
+    if (g.e.bias)
+        bias = dn_load_n<8>(static_cast<const T *>(g.e.bias) + col, n);
+    finish<T, true>(g.e, v, bias, row * g.J + col, row, col, n, seed);
 }
 
-// dbias from the shares of the column sums
+// dbias from the shares of the column sums: 16 columns a workgroup, 16 lanes a column
 template <class T>
-__global__ void __launch_bounds__(256) dense_colsum_join_kernel(const float *part, int splits, long long n, T *out)
+__global__ void __launch_bounds__(256) dense_colsum_join_kernel(const float *part, int parts, long long n, T *out)
 {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n)
-        return;
+    __shared__ float lds[16][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const long long i = (long long)blockIdx.x * 16 + x;
     float s = 0.f;
-    for (int k = 0; k < splits; ++k)
-        s += part[k * n + i];
-    out[i] = (T)s;
+    if (i < n) {
+#pragma unroll 4
+        for (int k = y; k < parts; k += 16)
+            s += part[k * n + i];
+    }
+    lds[y][x] = s;
+    __syncthreads();
+    if (y == 0 && i < n) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k)
+            s += lds[k][x];
+        out[i] = (T)s;
+    }
 }
 
 // Column sums of dz [M, N] by themselves (where dW is not wanted, or has no elements): 32 columns a workgroup
@@ -401,11 +530,25 @@ __global__ void __launch_bounds__(256) dense_colsum_kernel(const T *dz, long lon
 constexpr int CUS = 256;
 
 struct Plan {
-    int tile;                    // 0: 64 x 64, 1: 128 x 128
+    int tile;                    // index into TILES
     int tiles_i, tiles_j, splits, steps, steps_per_split;
     long long pitch;
     size_t bytes;                // of the fp32 shares
+    int sharers;                 // of the column sums
 };
+
+// The tiles a workgroup can make, rows x columns of C, the workgroups of a kind that fit a CU together (by LDS), its
+// waves side by side, and what a step of r costs one of them, in cycles, where the CU is full (16-bit types, fp32).
+struct TileKind {
+    int i, j, per_cu, waves_j, cost16, cost32;
+};
+constexpr TileKind TILES[] = {{64, 64, 4, 2, 330, 1350}, {128, 128, 2, 2, 800, 4700}, {256, 256, 1, 4, 2560, 18200}};
+
+// Which tile, and into how many shares r is cut: the cheapest by this estimate.  A CU works through its workgroups in
+// turns of as many as fit it; a step of r costs them together the cost above, and never less than the time a transfer
+// takes to arrive; a workgroup's start and end cost about as much as a few steps; shares are written, read and added by
+// a further kernel.
+constexpr double ARRIVE = 1400, START_END = 8000, JOIN = 8000, JOIN_BYTES = 2000;
 
 Plan plan(int type, long long I, long long J, long long R)
 {
@@ -414,21 +557,35 @@ Plan plan(int type, long long I, long long J, long long R)
     if (I < 1 || J < 1)
         return p;
     p.steps = (int)dn_ceil(R, type == OPUS_DENSE_F32 ? 32 : 64);
-    const long long big = dn_ceil(I, 128) * dn_ceil(J, 128);
-    p.tile = big >= CUS / 2 || (I > 64 && J > 64 && big * p.steps >= 4 * CUS) ? 1 : 0;
-    const int edge = p.tile ? 128 : 64;
-    p.tiles_i = (int)dn_ceil(I, edge);
-    p.tiles_j = (int)dn_ceil(J, edge);
-    const long long tiles = (long long)p.tiles_i * p.tiles_j;
-    // cut r until there are two workgroups a CU, but leave each at least four steps
-    long long splits = tiles >= CUS ? 1 : dn_ceil(2 * CUS, tiles);
-    if (splits > p.steps / 4)
-        splits = p.steps / 4;
-    if (splits < 1)
-        splits = 1;
-    p.steps_per_split = (int)dn_ceil(p.steps > 0 ? p.steps : 1, splits);
-    p.splits = p.steps > 0 ? (int)dn_ceil(p.steps, p.steps_per_split) : 1;
     p.pitch = dn_ceil(J, 8) * 8;
+    double best = 0;
+    for (int k = 0; k < 3; ++k) {
+        const TileKind &t = TILES[k];
+        const long long tiles = dn_ceil(I, t.i) * dn_ceil(J, t.j);
+        const int most = p.steps / 2 < 64 ? p.steps / 2 : 64;
+        for (int n = 1; n == 1 || n <= most; ++n) {
+            const long long each = dn_ceil(p.steps, n), blocks = tiles * n, a_cu = dn_ceil(blocks, CUS);
+            const long long together = a_cu < t.per_cu ? a_cu : t.per_cu, turns = dn_ceil(a_cu, together);
+            const double step = (double)together * (type == OPUS_DENSE_F32 ? t.cost32 : t.cost16);
+            double cost = turns * (each * (step > ARRIVE ? step : ARRIVE) + START_END);
+            if (n > 1)
+                cost += JOIN + 8.0 * n * I * p.pitch / JOIN_BYTES;
+            if (best == 0 || cost < best) {
+                best = cost;
+                p.tile = k;
+                p.splits = n;
+            }
+            if (blocks >= 4 * CUS * t.per_cu)
+                break;
+        }
+    }
+    const TileKind &t = TILES[p.tile];
+    p.tiles_i = (int)dn_ceil(I, t.i);
+    p.tiles_j = (int)dn_ceil(J, t.j);
+    p.steps_per_split = (int)dn_ceil(p.steps > 0 ? p.steps : 1, p.splits);
+    p.splits = p.steps > 0 ? (int)dn_ceil(p.steps, p.steps_per_split) : 1;
+    const int most = p.splits < 8 ? 8 / p.splits : 1;
+    p.sharers = (p.tiles_j < most ? p.tiles_j : most) * t.waves_j;
     p.bytes = p.splits > 1 ? (size_t)p.splits * I * p.pitch * sizeof(float) : 0;
     return p;
 }
@@ -439,13 +596,15 @@ template <class T, bool ARC, bool BRC, bool DIRECT>
 void launch_tiles(const Plan &p, const GemmArgs &g, hipStream_t s)
 {
     const dim3 grid((unsigned)(p.tiles_i * p.tiles_j * p.splits));
-    if (p.tile)
+    if (p.tile == 2)
+        hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 4, 4, 2, DIRECT>), grid, dim3(512), 0, s, g);
+    else if (p.tile == 1)
         hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 2, 2, 2, DIRECT>), grid, dim3(256), 0, s, g);
     else
         hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 2, 1, 1, DIRECT>), grid, dim3(256), 0, s, g);
 }
 
-// C = A B^T with an epilogue; `shares`: p.bytes of workspace.  colsum: [p.splits][I] fp32 or NULL.
+// C = A B^T with an epilogue; `shares`: p.bytes of workspace.  colsum: [p.splits * p.sharers][I] fp32 or NULL.
 template <class T, bool ARC, bool BRC>
 hipError_t gemm(int type, const void *a, const void *b, long long I, long long J, long long R, const Epilogue &e,
                 float *shares, float *colsum, hipStream_t s)
@@ -454,9 +613,12 @@ hipError_t gemm(int type, const void *a, const void *b, long long I, long long J
     if ((long long)p.tiles_i * p.tiles_j * p.splits * 256 > 0xFFFFFFFFll)
         return hipErrorInvalidValue;
     GemmArgs g = {a, b, I, J, R, p.tiles_i, p.tiles_j, p.splits, p.steps, p.steps_per_split,
-                  p.splits > 1 ? shares : nullptr, p.pitch, colsum, e};
+                  p.splits > 1 ? shares : nullptr, p.pitch, colsum, p.sharers, e};
     const int piece = Elem<T>::PIECE;
-    const bool direct = aligned16(a) && aligned16(b) && (ARC ? R : I) % piece == 0 && (BRC ? R : J) % piece == 0;
+    // (a tile's pieces are addressed in 32 bits from its corner)
+    const auto near = [](bool rc, long long i, long long r) { return (rc ? 256 * r : 64 * i) * sizeof(T) < (1ll << 31); };
+    const bool direct = aligned16(a) && aligned16(b) && (ARC ? R : I) % piece == 0 && (BRC ? R : J) % piece == 0 &&
+                        near(ARC, I, R) && near(BRC, J, R);
     if (direct)
         launch_tiles<T, ARC, BRC, true>(p, g, s);
     else
@@ -499,13 +661,13 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
         if (e != hipSuccess)
             return e;
         if (db)
-            hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 256)), dim3(256), 0, s, sums,
-                               p.splits, N, static_cast<T *>(db));
+            hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 16)), dim3(256), 0, s, sums,
+                               p.splits * p.sharers, N, static_cast<T *>(db));
     } else if (db && N) {
         const long long runs = colsum_runs(M, N), per = dn_ceil(M > 0 ? M : 1, runs);
         hipLaunchKernelGGL(dense_colsum_kernel<T>, dim3((unsigned)dn_ceil(N, 32), (unsigned)runs), dim3(256), 0, s,
                            static_cast<const T *>(dz), M, N, per, ws);
-        hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 256)), dim3(256), 0, s, ws,
+        hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 16)), dim3(256), 0, s, ws,
                            (int)runs, N, static_cast<T *>(db));
     }
     return hipSuccess;
@@ -538,7 +700,7 @@ size_t dn_linear_backward_workspace(int type, long long M, long long N, long lon
         return 0;
     const size_t x = M > 0 && K > 0 ? plan(type, M, K, N).bytes : 0;
     const Plan p = plan(type, N, K, M);
-    const size_t w = align256(p.bytes) + (size_t)p.splits * N * sizeof(float);
+    const size_t w = align256(p.bytes) + (size_t)p.splits * p.sharers * N * sizeof(float);
     const size_t alone = (size_t)colsum_runs(M, N) * N * sizeof(float);
     const size_t most = x > w ? x : w;
     return most > alone ? most : alone;

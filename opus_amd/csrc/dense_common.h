@@ -27,32 +27,81 @@ template <int N, class T> __device__ __forceinline__ void dn_store(T *p, typenam
     *reinterpret_cast<typename DnVec<T, N>::at *>(p) = v;
 }
 
-// Up to N elements as floats: all N where `n` >= N, zeros beyond `n` otherwise.
-template <int N, class T> __device__ __forceinline__ dn_floats<N> dn_load_n(const T *p, int n)
+// The n elements at p, 0 < n < N, and zeros: the vector that ends with them, shifted down.  N - n elements before p
+// have to be readable (the row has N elements or more).
+template <int N, class T> __device__ __forceinline__ typename DnVec<T, N>::type dn_load_tail(const T *p, int n)
 {
-    dn_floats<N> r = 0.f;
-    if (n >= N) {
-        r = __builtin_convertvector(dn_load<N>(p), dn_floats<N>);
-    } else {
+    constexpr int W = N * sizeof(T) / 4;
+    typedef uint32_t words __attribute__((ext_vector_type(W)));
+    const int skip = N - n;
+    words a = __builtin_bit_cast(words, dn_load<N>(p - skip));
+    const int whole = sizeof(T) == 4 ? skip : skip >> 1;
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < n)
-                r[j] = (float)p[j];
+    for (int b = W / 2; b; b /= 2)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            a[i] = whole & b ? (i + b < W ? a[i + b] : 0u) : a[i];
+    if (sizeof(T) == 2)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            a[i] = skip & 1 ? (uint32_t)(((i + 1 < W ? (uint64_t)a[i + 1] << 32 : 0) | a[i]) >> 16) : a[i];
+    return __builtin_bit_cast(typename DnVec<T, N>::type, a);
+}
+
+// Up to N elements: all N where `n` >= N, zeros beyond `n` otherwise.  `row`: how many the whole row has.  WHOLE: n is
+// no less than N if it is positive at all.
+template <int N, bool WHOLE = false, class T>
+__device__ __forceinline__ typename DnVec<T, N>::type dn_load_raw(const T *p, int n, int row)
+{
+    typename DnVec<T, N>::type r = (T)0.f;
+    if (WHOLE) {
+        if (n > 0)
+            r = dn_load<N>(p);
+    } else if (n >= N) {
+        r = dn_load<N>(p);
+    } else if (n > 0) {
+        if (row >= N) {
+            r = dn_load_tail<N>(p, n);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < n)
+                    r[j] = p[j];
+        }
     }
     return r;
 }
+template <int N, bool WHOLE = false, class T>
+__device__ __forceinline__ dn_floats<N> dn_load_n(const T *p, int n, int row)
+{
+    return __builtin_convertvector(dn_load_raw<N, WHOLE>(p, n, row), dn_floats<N>);
+}
 
 // The first `n` of N floats, each rounded to T once, to nearest even.
-template <int N, class T> __device__ __forceinline__ void dn_store_n(T *p, dn_floats<N> v, int n)
+template <int N, bool WHOLE = false, class T> __device__ __forceinline__ void dn_store_n(T *p, dn_floats<N> v, int n)
 {
-    const typename DnVec<T, N>::type r = __builtin_convertvector(v, typename DnVec<T, N>::type);
-    if (n >= N) {
+    typename DnVec<T, N>::type r = __builtin_convertvector(v, typename DnVec<T, N>::type);
+    if (WHOLE) {
+        if (n > 0)
+            dn_store<N>(p, r);
+    } else if (n >= N) {
         dn_store<N>(p, r);
-    } else {
+    } else if (n > 0) {
+        // halves, quarters, ... of the vector, the stored part shifted out each time
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < n)
-                p[j] = r[j];
+        for (int b = N / 2; b; b /= 2)
+            if (n & b) {
+                if (b == 4)
+                    dn_store<4>(p, __builtin_shufflevector(r, r, 0, 1, 2, 3));
+                else if (b == 2)
+                    dn_store<2>(p, __builtin_shufflevector(r, r, 0, 1));
+                else
+                    p[0] = r[0];
+                p += b;
+#pragma unroll
+                for (int j = 0; j + b < N; ++j)
+                    r[j] = r[j + b];
+            }
     }
 }
 

@@ -33,13 +33,13 @@ __global__ void __launch_bounds__(EW_THREADS) dense_elementwise_kernel(EwArgs a)
         return;
     const uint64_t at = row * a.cols + col;
     const int n = (int)min(8u, a.cols - col);
-    dn_floats<8> v = dn_load_n<8>(static_cast<const T *>(a.x) + at, n);
+    dn_floats<8> v = dn_load_n<8>(static_cast<const T *>(a.x) + at, n, (int)a.cols);
     if (a.drop.threshold)
         dn_drop<8>(v, row, col, seed, a.drop);
     if constexpr (SLOPE) {
-        dn_act_slope<8>(v, dn_load_n<8>(static_cast<const T *>(a.slope) + at, n), a.act);
+        dn_act_slope<8>(v, dn_load_n<8>(static_cast<const T *>(a.slope) + at, n, (int)a.cols), a.act);
     } else if (a.residual) {
-        v += dn_load_n<8>(static_cast<const T *>(a.residual) + at, n);
+        v += dn_load_n<8>(static_cast<const T *>(a.residual) + at, n, (int)a.cols);
     }
     dn_store_n<8>(static_cast<T *>(a.y) + at, v, n);
 }

@@ -39,11 +39,11 @@ struct Epilogue {
     DnDrop drop;
 };
 
-// v: eight values of C at (row, col ..), element `at` of y, `n` of them inside (all of them, where !EDGE); col is a
+// v: eight values of C at (row, col ..), element `at` of y, `n` of them inside its `cols` columns (all of them, where !EDGE); col is a
 // multiple of 8.  bias: those columns' (zeros without one).
 template <class T, bool EDGE>
 __device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, const dn_floats<8> &bias, uint64_t at, uint64_t row,
-                                       uint32_t col, int n, uint64_t seed)
+                                       uint32_t col, int n, int cols, uint64_t seed)
 {
     if (!EDGE)
         n = 8;
@@ -62,7 +62,7 @@ __device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, const 
     if (e.drop.threshold)
         dn_drop<8>(v, row, col, seed, e.drop);
     if (e.residual)
-        v += dn_load_n<8>(static_cast<const T *>(e.residual) + at, n);
+        v += dn_load_n<8>(static_cast<const T *>(e.residual) + at, n, cols);
     dn_store_n<8>(static_cast<T *>(e.y) + at, v, n);
 }
 
@@ -163,18 +163,10 @@ struct Tile {
         for (int t = 0; t < PIECES / THREADS; ++t) {
             int w, r;
             coords(t * THREADS + tid, w, r);
-            v[t] = (T)0.f;
             const long long i = w0 + w, rr = r0 + r;
             const T *src = RC ? base + i * R + rr : base + rr * I + i;
             const long long inside = RC ? (i < I ? R - rr : 0) : (rr < R ? I - i : 0);
-            if (inside >= PIECE) {
-                v[t] = dn_load<PIECE>(src);
-            } else {
-#pragma unroll
-                for (int j = 0; j < PIECE; ++j)
-                    if (j < inside)
-                        v[t][j] = src[j];
-            }
+            v[t] = dn_load_raw<PIECE>(src, (int)max(-1ll, min(inside, (long long)PIECE)), (int)min((long long)PIECE, RC ? R : I));
         }
     }
     template <int THREADS> static __device__ __forceinline__ void write(const Pieces<THREADS> &v, char *lds, int tid)
@@ -439,17 +431,17 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
             const int n = (int)min(8ll, g.J - cj);
             dn_floats<8> bias = 0.f;
             if (g.e.bias)
-                bias = dn_load_n<8>(static_cast<const T *>(g.e.bias) + cj, n);
+                bias = dn_load_n<8>(static_cast<const T *>(g.e.bias) + cj, n, (int)g.J);
             uint64_t at = (uint64_t)ci * g.J + cj;
             if (inside) {
 #pragma unroll
                 for (int q = 0; q < 32 / RPT; ++q, at += RPT * g.J)
-                    finish<T, false>(g.e, value(q), bias, at, ci + q * RPT, (uint32_t)cj, 8, seed);
+                    finish<T, false>(g.e, value(q), bias, at, ci + q * RPT, (uint32_t)cj, 8, (int)g.J, seed);
             } else {
 #pragma unroll 1
                 for (int q = 0; q < 32 / RPT; ++q, at += RPT * g.J)
                     if (ci + q * RPT < g.I && n > 0)
-                        finish<T, true>(g.e, value(q), bias, at, ci + q * RPT, (uint32_t)cj, n, seed);
+                        finish<T, true>(g.e, value(q), bias, at, ci + q * RPT, (uint32_t)cj, n, (int)g.J, seed);
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -475,8 +467,8 @@ __global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g)
     const int n = (int)min(8ll, g.J - (long long)col);
     dn_floats<8> bias = 0.f;
     if (g.e.bias)
-        bias = dn_load_n<8>(static_cast<const T *>(g.e.bias) + col, n);
-    finish<T, true>(g.e, v, bias, row * g.J + col, row, col, n, seed);
+        bias = dn_load_n<8>(static_cast<const T *>(g.e.bias) + col, n, (int)g.J);
+    finish<T, true>(g.e, v, bias, row * g.J + col, row, col, n, (int)g.J, seed);
 }
 
 // dbias from the shares of the column sums: 16 columns a workgroup, 16 lanes a column

@@ -3,8 +3,8 @@
 // Bound by memory: forward two reads and up to two writes an element, backward four reads and two writes.  A row is
 // read once and stays in registers: TPR threads share it, each holding CH runs of VEC consecutive elements, so the
 // mean, the sum of squared deviations from it (two passes over registers, not over memory: no cancellation) and the
-// results cost no second read.  A wave takes a row of up to 1024 elements by itself (sums by lane exchange alone);
-// wider rows take 4, 8 or 16 waves and one LDS exchange a sum.
+// results cost no second read.  A wave takes a row of up to 512 elements by itself (sums by lane exchange alone);
+// wider rows take 2 to 16 waves and one LDS exchange a sum.
 //
 // Backward: r, and with a post-norm the block's normed rows, are computed again from x and block with the forward's
 // statistics.  Sums over rows (dweight, dbias, dpost_*, dgate) stay in each thread's registers while its workgroup
@@ -60,26 +60,51 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float *lds, int &phase)
 }
 
 template <int CH, int VEC> using Row = dn_floats<VEC>[CH];
+template <class T, int CH, int VEC> using Raw = typename DnVec<T, VEC>::type[CH];       // a row as it lies in memory
 
-template <class T, int TPR, int VEC, int CH>
-__device__ __forceinline__ void load_row(Row<CH, VEC> &r, const T *p, int lane, int width)
+template <class T, int TPR, int VEC, int CH, bool WHOLE>
+__device__ __forceinline__ void load_row(Raw<T, CH, VEC> &r, const T *p, int lane, int width)
 {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * TPR + lane) * VEC;
-        r[c] = dn_load_n<VEC>(p + col, width - col);
+        r[c] = dn_load_raw<VEC, WHOLE>(p + col, width - col, width);
     }
 }
 
-template <class T, int TPR, int VEC, int CH>
+template <class T, int TPR, int VEC, int CH, bool WHOLE>
 __device__ __forceinline__ void store_row(T *p, const Row<CH, VEC> &r, int lane, int width)
 {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * TPR + lane) * VEC;
-        dn_store_n<VEC>(p + col, r[c], width - col);
+        dn_store_n<VEC, WHOLE>(p + col, r[c], width - col);
     }
 }
+
+// A vector of `width` that every row uses: held in registers where a thread's part is small (KEEP), else loaded again
+// (from the caches) for every row.
+template <class T, int TPR, int VEC, int CH, bool WHOLE, bool KEEP>
+struct Param {
+    Raw<T, KEEP ? CH : 1, VEC> held;
+    const T *p;
+    __device__ __forceinline__ Param(const void *from, int lane, int width) : p(static_cast<const T *>(from))
+    {
+        if constexpr (KEEP)
+            if (p)
+                load_row<T, TPR, VEC, CH, WHOLE>(held, p, lane, width);
+    }
+    __device__ __forceinline__ explicit operator bool() const { return p; }
+    __device__ __forceinline__ dn_floats<VEC> at(int c, int lane, int width) const
+    {
+        if constexpr (KEEP) {
+            return __builtin_convertvector(held[c], dn_floats<VEC>);
+        } else {
+            const int col = (c * TPR + lane) * VEC;
+            return dn_load_n<VEC, WHOLE>(p + col, width - col, width);
+        }
+    }
+};
 
 // mean (0 for RMS) and 1 / sigma of a row in registers (zeros beyond `width`)
 template <int TPR, int VEC, int CH>
@@ -111,168 +136,204 @@ __device__ __forceinline__ void row_stats(const Row<CH, VEC> &r, int lane, const
     rstd = 1.f / sqrtf(s[0] * a.inv_width + a.eps);
 }
 
-constexpr int group_threads(int TPR) { return TPR < 256 ? 256 : TPR; }
+constexpr int group_threads(int TPR) { return TPR < 128 ? 256 : TPR; }
 
-template <class T, int TPR, int VEC, int CH>
+// The next row's values are on their way while a row is worked on.
+template <class T, int TPR, int VEC, int CH, bool WHOLE>
 __global__ void __launch_bounds__(group_threads(TPR)) dense_norm_forward_kernel(NormArgs a)
 {
     constexpr int ROWS = group_threads(TPR) / TPR;
+    constexpr bool KEEP = sizeof(T) * VEC * CH <= 16;
     __shared__ float lds[64];
     int phase = 0;
     const int lane = threadIdx.x % TPR, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
-    const uint64_t seed = dn_seed(a.drop);
-    const T *weight = static_cast<const T *>(a.weight), *bias = static_cast<const T *>(a.bias);
-    const T *pw = static_cast<const T *>(a.post_weight), *pb = static_cast<const T *>(a.post_bias);
     // every thread of a workgroup makes the same number of turns (the sums have barriers where TPR > 64, and then
     // ROWS is 1)
-    for (long long row = (long long)blockIdx.x * ROWS + sub; row < a.rows; row += (long long)gridDim.x * ROWS) {
+    const long long first = (long long)blockIdx.x * ROWS + sub, stride = (long long)gridDim.x * ROWS;
+    if (first >= a.rows)
+        return;
+    const uint64_t seed = dn_seed(a.drop);
+    const T *x = static_cast<const T *>(a.x), *block = static_cast<const T *>(a.block);
+    Raw<T, CH, VEC> next_h, next_x;
+    load_row<T, TPR, VEC, CH, WHOLE>(next_h, block + first * a.width, lane, a.width);
+    load_row<T, TPR, VEC, CH, WHOLE>(next_x, x + first * a.width, lane, a.width);
+    using P = Param<T, TPR, VEC, CH, WHOLE, KEEP>;
+    const P weight(a.weight, lane, a.width), bias(a.bias, lane, a.width);
+    const P pw(a.post_weight, lane, a.width), pb(a.post_bias, lane, a.width);
+    for (long long row = first; row < a.rows; row += stride) {
         const long long at = row * a.width;
         Row<CH, VEC> h, r;
-        load_row<T, TPR, VEC, CH>(h, static_cast<const T *>(a.block) + at, lane, a.width);
-        load_row<T, TPR, VEC, CH>(r, static_cast<const T *>(a.x) + at, lane, a.width);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            h[c] = __builtin_convertvector(next_h[c], dn_floats<VEC>);
+            r[c] = __builtin_convertvector(next_x[c], dn_floats<VEC>);
+        }
+        if (row + stride < a.rows) {
+            load_row<T, TPR, VEC, CH, WHOLE>(next_h, block + at + stride * a.width, lane, a.width);
+            load_row<T, TPR, VEC, CH, WHOLE>(next_x, x + at + stride * a.width, lane, a.width);
+        }
         float mean2 = 0.f, rstd2 = 1.f, mean, rstd;
+        const T *gate = a.gate ? static_cast<const T *>(a.gate) + row / a.rows_per_gate * a.width : nullptr;
         if (pw)
             row_stats<TPR, VEC, CH>(h, lane, a, lds, phase, mean2, rstd2);
-        const T *gate = a.gate ? static_cast<const T *>(a.gate) + row / a.rows_per_gate * a.width : nullptr;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int col = (c * TPR + lane) * VEC, n = a.width - col;
             dn_floats<VEC> u = h[c];
             if (pw) {
-                u = (u - mean2) * rstd2 * dn_load_n<VEC>(pw + col, n);
+                u = (u - mean2) * rstd2 * pw.at(c, lane, a.width);
                 if (pb)
-                    u += dn_load_n<VEC>(pb + col, n);
+                    u += pb.at(c, lane, a.width);
             }
             if (a.drop.threshold)
                 dn_drop<VEC>(u, row, col, seed, a.drop);
             if (gate)
-                u *= dn_load_n<VEC>(gate + col, n);
+                u *= dn_load_n<VEC, WHOLE>(gate + col, n, a.width);
             r[c] = r[c] * a.scale + u;
-            if (n < VEC)                           // what lies beyond the row stays out of its sums
+            if (!WHOLE && n < VEC)                 // what lies beyond the row stays out of its sums
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
                     r[c][j] = j < n ? r[c][j] : 0.f;
         }
         if (a.stream_out)
-            store_row<T, TPR, VEC, CH>(static_cast<T *>(a.stream_out) + at, r, lane, a.width);
+            store_row<T, TPR, VEC, CH, WHOLE>(static_cast<T *>(a.stream_out) + at, r, lane, a.width);
         row_stats<TPR, VEC, CH>(r, lane, a, lds, phase, mean, rstd);
-        if (a.stats && lane == 0) {
-            float4 st = make_float4(mean2, rstd2, mean, rstd);
-            *reinterpret_cast<float4 *>(a.stats + row * 4) = st;
-        }
+        if (a.stats && lane == 0)
+            *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(mean2, rstd2, mean, rstd);
         if (a.y) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int col = (c * TPR + lane) * VEC, n = a.width - col;
                 r[c] = (r[c] - mean) * rstd;
                 if (weight)
-                    r[c] *= dn_load_n<VEC>(weight + col, n);
+                    r[c] *= weight.at(c, lane, a.width);
                 if (bias)
-                    r[c] += dn_load_n<VEC>(bias + col, n);
+                    r[c] += bias.at(c, lane, a.width);
             }
-            store_row<T, TPR, VEC, CH>(static_cast<T *>(a.y) + at, r, lane, a.width);
+            store_row<T, TPR, VEC, CH, WHOLE>(static_cast<T *>(a.y) + at, r, lane, a.width);
         }
     }
 }
 
 // Adds `acc` of the workgroup's ROWS row lanes and stores it as one row of `width` floats (or of T).
-template <class O, int TPR, int VEC, int CH>
+template <class O, int TPR, int VEC, int CH, bool WHOLE>
 __device__ __forceinline__ void flush(O *out, Row<CH, VEC> &acc, float *cols, int lane, int sub, int width)
 {
     constexpr int ROWS = group_threads(TPR) / TPR;
     if constexpr (ROWS == 1) {
-        store_row<O, TPR, VEC, CH>(out, acc, lane, width);
+        store_row<O, TPR, VEC, CH, WHOLE>(out, acc, lane, width);
     } else {
+        static_assert(CH == 1, "the first row's threads add a whole row");
         __syncthreads();
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-            *reinterpret_cast<dn_floats<VEC> *>(cols + ((sub * CH + c) * TPR + lane) * VEC) = acc[c];
+        *reinterpret_cast<dn_floats<VEC> *>(cols + (sub * TPR + lane) * VEC) = acc[0];
         __syncthreads();
-        // the first CH rows' worth of threads: CH <= ROWS, thread (sub, lane) adds run `sub`
-        static_assert(CH <= ROWS, "one turn covers a row");
-        if (sub < CH) {
-            dn_floats<VEC> t = 0.f;
+        if (sub == 0) {
+            dn_floats<VEC> t = acc[0];
 #pragma unroll
-            for (int w = 0; w < ROWS; ++w)
-                t += *reinterpret_cast<const dn_floats<VEC> *>(cols + ((w * CH + sub) * TPR + lane) * VEC);
-            const int col = (sub * TPR + lane) * VEC;
-            dn_store_n<VEC>(out + col, t, width - col);
+            for (int w = 1; w < ROWS; ++w)
+                t += *reinterpret_cast<const dn_floats<VEC> *>(cols + (w * TPR + lane) * VEC);
+            dn_store_n<VEC, WHOLE>(out + lane * VEC, t, width - lane * VEC);
         }
     }
 }
 
-// POST: with a post-norm.  Workgroup (g, k): rows k * rows_per_group .. of gate row g where chunks > 1 or the gate
-// has one row; otherwise rows_per_group whole gate rows.
-template <class T, int TPR, int VEC, int CH, bool POST>
+// POST: with a post-norm.  BIAS: a bias' gradient may be wanted.  A workgroup works on rows_per_group consecutive rows of one gate row where chunks > 1,
+// otherwise on rows_per_group whole gate rows.  The next row's values are on their way while a row is worked on.
+template <class T, int TPR, int VEC, int CH, bool WHOLE, bool POST, bool BIAS>
 __global__ void __launch_bounds__(group_threads(TPR)) dense_norm_backward_kernel(NormArgs a)
 {
     constexpr int ROWS = group_threads(TPR) / TPR;
+    constexpr bool KEEP = sizeof(T) * VEC * CH <= 16, AHEAD = CH == 1 || (TPR < 1024 && sizeof(T) == 2);
     __shared__ float lds[64];
-    __shared__ __align__(16) float cols[ROWS > 1 ? ROWS * CH * TPR * VEC : 4];
+    __shared__ __align__(16) float cols[ROWS > 1 ? ROWS * TPR * VEC : 4];
     int phase = 0;
-    const int lane = threadIdx.x % TPR, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+    const int lane = threadIdx.x % TPR, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), width = a.width;
     const uint64_t seed = dn_seed(a.drop);
-    const T *weight = static_cast<const T *>(a.weight);
-    const T *pw = static_cast<const T *>(a.post_weight), *pb = static_cast<const T *>(a.post_bias);
+    const T *x = static_cast<const T *>(a.x), *block = static_cast<const T *>(a.block);
+    const T *dy_in = static_cast<const T *>(a.dy), *ds_in = static_cast<const T *>(a.dstream);
 
     Row<CH, VEC> dw, db, dpw, dpb, dg;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
         dw[c] = db[c] = dpw[c] = dpb[c] = dg[c] = 0.f;
 
-    long long g0, g1, chunk = 0;
+    // rows first .. last of gate rows g0 .. g1
+    long long g0, g1, first, last;
     if (a.chunks > 1) {
         g0 = blockIdx.x / a.chunks;
         g1 = g0 + 1;
-        chunk = blockIdx.x - g0 * a.chunks;
+        first = g0 * a.rows_per_gate + (blockIdx.x - g0 * a.chunks) * a.rows_per_group;
+        last = min(first + a.rows_per_group, g1 * a.rows_per_gate);
     } else {
         g0 = blockIdx.x * a.rows_per_group;
         g1 = min(g0 + a.rows_per_group, a.gate_rows);
+        first = g0 * a.rows_per_gate;
+        last = g1 * a.rows_per_gate;
     }
+    Raw<T, CH, VEC> raw_h, raw_x, raw_dy, raw_ds;
+    float4 raw_st = make_float4(0.f, 1.f, 0.f, 1.f);
+    const auto load = [&](long long row) __attribute__((always_inline)) {
+        const long long at = row * width;
+        load_row<T, TPR, VEC, CH, WHOLE>(raw_h, block + at, lane, width);
+        load_row<T, TPR, VEC, CH, WHOLE>(raw_x, x + at, lane, width);
+        if (dy_in)
+            load_row<T, TPR, VEC, CH, WHOLE>(raw_dy, dy_in + at, lane, width);
+        if (ds_in)
+            load_row<T, TPR, VEC, CH, WHOLE>(raw_ds, ds_in + at, lane, width);
+        raw_st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+    };
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        raw_dy[c] = raw_ds[c] = (T)0.f;
+    if (AHEAD && first + sub < last)
+        load(first + sub);
+    using P = Param<T, TPR, VEC, CH, WHOLE, KEEP>;
+    const P weight(a.weight, lane, width), pw(POST ? a.post_weight : nullptr, lane, width), pb(POST ? a.post_bias : nullptr, lane, width);
+
+    long long row = first + sub;
     for (long long g = g0; g < g1; ++g) {
-        long long first = g * a.rows_per_gate, last = first + a.rows_per_gate;
-        if (a.chunks > 1) {
-            first += chunk * a.rows_per_group;
-            last = min(first + a.rows_per_group, last);
-        }
-        const T *gate = a.gate ? static_cast<const T *>(a.gate) + g * a.width : nullptr;
-        for (long long row = first + sub; row < last; row += ROWS) {
-            const long long at = row * a.width;
+        const long long end = min((g + 1) * a.rows_per_gate, last);
+        const T *gate = a.gate ? static_cast<const T *>(a.gate) + g * width : nullptr;
+        for (; row < end; row += ROWS) {
+            const long long at = row * width;
             if (a.gate_per_row)
                 gate = static_cast<const T *>(a.gate) + at;
+            if (!AHEAD)
+                load(row);
             Row<CH, VEC> h, r, dy;
-            load_row<T, TPR, VEC, CH>(h, static_cast<const T *>(a.block) + at, lane, a.width);
-            load_row<T, TPR, VEC, CH>(r, static_cast<const T *>(a.x) + at, lane, a.width);
-            if (a.dy) {
-                load_row<T, TPR, VEC, CH>(dy, static_cast<const T *>(a.dy) + at, lane, a.width);
-            } else {
+            Raw<T, CH, VEC> ds;
+            const float4 st = raw_st;
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-                    dy[c] = 0.f;
+            for (int c = 0; c < CH; ++c) {
+                h[c] = __builtin_convertvector(raw_h[c], dn_floats<VEC>);
+                r[c] = __builtin_convertvector(raw_x[c], dn_floats<VEC>);
+                dy[c] = __builtin_convertvector(raw_dy[c], dn_floats<VEC>);
+                ds[c] = raw_ds[c];
             }
-            const float4 st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+            if (AHEAD && row + ROWS < last)
+                load(row + ROWS);
             // xhat in r, D(post(block)) in u
             float s[2] = {0.f, 0.f};
             Row<CH, VEC> u;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int col = (c * TPR + lane) * VEC, n = a.width - col;
+                const int col = (c * TPR + lane) * VEC, n = width - col;
                 if constexpr (POST) {
                     h[c] = (h[c] - st.x) * st.y;                        // hhat
-                    u[c] = h[c] * dn_load_n<VEC>(pw + col, n);
+                    u[c] = h[c] * pw.at(c, lane, width);
                     if (pb)
-                        u[c] += dn_load_n<VEC>(pb + col, n);
+                        u[c] += pb.at(c, lane, width);
                 } else {
                     u[c] = h[c];
                 }
                 if (a.drop.threshold)
                     dn_drop<VEC>(u[c], row, col, seed, a.drop);
-                r[c] = r[c] * a.scale + (gate ? u[c] * dn_load_n<VEC>(gate + col, n) : u[c]);
+                r[c] = r[c] * a.scale + (gate ? u[c] * dn_load_n<VEC, WHOLE>(gate + col, n, width) : u[c]);
                 r[c] = (r[c] - st.z) * st.w;
                 dw[c] += dy[c] * r[c];
-                db[c] += dy[c];
+                if constexpr (BIAS)
+                    db[c] += dy[c];
                 if (weight)
-                    dy[c] *= dn_load_n<VEC>(weight + col, n);
+                    dy[c] *= weight.at(c, lane, width);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {                         // (dy is zero beyond the row)
                     s[0] += dy[c][j];
@@ -284,32 +345,31 @@ __global__ void __launch_bounds__(group_threads(TPR)) dense_norm_backward_kernel
             float t[2] = {0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int col = (c * TPR + lane) * VEC, n = a.width - col;
-                dn_floats<VEC> dr = st.w * (dy[c] - m0 - r[c] * m1);
-                if (a.dstream)
-                    dr += dn_load_n<VEC>(static_cast<const T *>(a.dstream) + at + col, n);
-                if (a.dx && n > 0)
-                    dn_store_n<VEC>(static_cast<T *>(a.dx) + at + col, dr * a.scale, n);
+                const int col = (c * TPR + lane) * VEC, n = width - col;
+                dn_floats<VEC> dr = st.w * (dy[c] - m0 - r[c] * m1) + __builtin_convertvector(ds[c], dn_floats<VEC>);
+                if (a.dx)
+                    dn_store_n<VEC, WHOLE>(static_cast<T *>(a.dx) + at + col, dr * a.scale, n);
                 if (gate) {
                     const dn_floats<VEC> dgate = dr * u[c];
                     dg[c] += dgate;
-                    if (a.dgate && a.gate_per_row && n > 0)
-                        dn_store_n<VEC>(static_cast<T *>(a.dgate) + at + col, dgate, n);
-                    dr *= dn_load_n<VEC>(gate + col, n);
+                    if (a.dgate && a.gate_per_row)
+                        dn_store_n<VEC, WHOLE>(static_cast<T *>(a.dgate) + at + col, dgate, n);
+                    dr *= dn_load_n<VEC, WHOLE>(gate + col, n, width);
                 }
                 if (a.drop.threshold)
                     dn_drop<VEC>(dr, row, col, seed, a.drop);
                 if constexpr (POST) {
                     dpw[c] += dr * h[c];
-                    dpb[c] += dr;
-                    u[c] = dr * dn_load_n<VEC>(pw + col, n);
+                    if constexpr (BIAS)
+                        dpb[c] += dr;
+                    u[c] = dr * pw.at(c, lane, width);
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
                         t[0] += u[c][j];
                         t[1] += u[c][j] * h[c][j];
                     }
-                } else if (a.dblock && n > 0) {
-                    dn_store_n<VEC>(static_cast<T *>(a.dblock) + at + col, dr, n);
+                } else if (a.dblock) {
+                    dn_store_n<VEC, WHOLE>(static_cast<T *>(a.dblock) + at + col, dr, n);
                 }
             }
             if constexpr (POST) {
@@ -319,35 +379,35 @@ __global__ void __launch_bounds__(group_threads(TPR)) dense_norm_backward_kernel
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
                         u[c] = st.y * (u[c] - n0 - h[c] * n1);
-                    store_row<T, TPR, VEC, CH>(static_cast<T *>(a.dblock) + at, u, lane, a.width);
+                    store_row<T, TPR, VEC, CH, WHOLE>(static_cast<T *>(a.dblock) + at, u, lane, width);
                 }
             }
         }
         if (gate && !a.gate_per_row) {
             if (a.part_gate)
-                flush<float, TPR, VEC, CH>(a.part_gate + (long long)blockIdx.x * a.width, dg, cols, lane, sub, a.width);
+                flush<float, TPR, VEC, CH, WHOLE>(a.part_gate + (long long)blockIdx.x * width, dg, cols, lane, sub, width);
             else if (a.dgate)
-                flush<T, TPR, VEC, CH>(static_cast<T *>(a.dgate) + g * a.width, dg, cols, lane, sub, a.width);
+                flush<T, TPR, VEC, CH, WHOLE>(static_cast<T *>(a.dgate) + g * width, dg, cols, lane, sub, width);
 #pragma unroll
             for (int c = 0; c < CH; ++c)
                 dg[c] = 0.f;
         }
     }
-    const long long mine = (long long)blockIdx.x * a.width;
+    const long long mine = (long long)blockIdx.x * width;
     if (a.part_w)
-        flush<float, TPR, VEC, CH>(a.part_w + mine, dw, cols, lane, sub, a.width);
-    if (a.part_b)
-        flush<float, TPR, VEC, CH>(a.part_b + mine, db, cols, lane, sub, a.width);
+        flush<float, TPR, VEC, CH, WHOLE>(a.part_w + mine, dw, cols, lane, sub, width);
+    if (BIAS && a.part_b)
+        flush<float, TPR, VEC, CH, WHOLE>(a.part_b + mine, db, cols, lane, sub, width);
     if constexpr (POST) {
         if (a.part_pw)
-            flush<float, TPR, VEC, CH>(a.part_pw + mine, dpw, cols, lane, sub, a.width);
-        if (a.part_pb)
-            flush<float, TPR, VEC, CH>(a.part_pb + mine, dpb, cols, lane, sub, a.width);
+            flush<float, TPR, VEC, CH, WHOLE>(a.part_pw + mine, dpw, cols, lane, sub, width);
+        if (BIAS && a.part_pb)
+            flush<float, TPR, VEC, CH, WHOLE>(a.part_pb + mine, dpb, cols, lane, sub, width);
     }
 }
 
 // out[g, col] = sum of part[g * count .. +count][col], for up to five tensors (blockIdx.z) of one row and the gate's
-// of gate_rows.  32 columns a workgroup, eight row lanes that are added in LDS.
+// of gate_rows.  16 columns a workgroup, 16 row lanes that are added in LDS.
 struct ReduceArgs {
     const float *part[5];
     void *out[5];
@@ -359,19 +419,21 @@ struct ReduceArgs {
 template <class T>
 __global__ void __launch_bounds__(256) dense_reduce_rows_kernel(ReduceArgs a)
 {
-    __shared__ float lds[8][33];
-    const int z = blockIdx.z, x = threadIdx.x & 31, y = threadIdx.x >> 5, col = blockIdx.x * 32 + x;
+    __shared__ float lds[16][17];
+    const int z = blockIdx.z, x = threadIdx.x & 15, y = threadIdx.x >> 4, col = blockIdx.x * 16 + x;
     for (long long g = blockIdx.y; g < a.groups[z]; g += gridDim.y) {
         const long long first = g * a.count[z], last = first + a.count[z];
         float s = 0.f;
-        if (col < a.width)
-            for (long long i = first + y; i < last; i += 8)
+        if (col < a.width) {
+#pragma unroll 8
+            for (long long i = first + y; i < last; i += 16)
                 s += a.part[z][i * a.width + col];
+        }
         lds[y][x] = s;
         __syncthreads();
         if (y == 0 && col < a.width) {
 #pragma unroll
-            for (int i = 1; i < 8; ++i)
+            for (int i = 1; i < 16; ++i)
                 s += lds[i][x];
             static_cast<T *>(a.out[z])[g * a.width + col] = (T)s;
         }
@@ -387,14 +449,16 @@ struct NormPlan {
 
 int threads_per_row(long long width)
 {
-    return width <= 1024 ? 64 : width <= 4096 ? 256 : width <= 8192 ? 512 : 1024;
+    return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 2048 ? 256 : width <= 8192 ? 512 : 1024;
 }
 
 NormPlan plan_backward(long long rows, long long width, long long gate_rows)
 {
     const int tpr = threads_per_row(width), lanes = group_threads(tpr) / tpr;
-    // two workgroups a CU hide each other's latency; more would only lengthen the second kernel's sums
-    const long long target = tpr <= 256 ? 512 : 256;
+    // 16 waves a CU hide each other's latency (8 of the widest kinds fill its registers); more workgroups, or ones of
+    // fewer than four rows a wave, would only lengthen the second kernel's sums
+    const long long full = width > 4096 ? 256 : 256 * (1024 / group_threads(tpr)), worth = dn_ceil(rows, 4 * lanes);
+    const long long target = full < worth ? full : worth;
     NormPlan p;
     if (rows < 1) {                      // nothing to add: every sum is empty
         p = {gate_rows > 0 ? gate_rows : 1, 0, 0, 0, 1};
@@ -419,38 +483,49 @@ NormPlan plan_backward(long long rows, long long width, long long gate_rows)
     return p;
 }
 
-template <class T, int TPR, int VEC, int CH>
+template <class T, int TPR, int VEC, int CH, bool WHOLE>
 void launch_forward(const NormArgs &a, hipStream_t s)
 {
     constexpr int ROWS = group_threads(TPR) / TPR;
     const long long blocks = dn_ceil(a.rows, ROWS);
     const unsigned grid = (unsigned)(blocks < 2048 ? blocks : 2048);
-    hipLaunchKernelGGL((dense_norm_forward_kernel<T, TPR, VEC, CH>), dim3(grid), dim3(group_threads(TPR)), 0, s, a);
+    hipLaunchKernelGGL((dense_norm_forward_kernel<T, TPR, VEC, CH, WHOLE>), dim3(grid), dim3(group_threads(TPR)), 0, s, a);
 }
 
-template <class T, int TPR, int VEC, int CH>
+template <class T, int TPR, int VEC, int CH, bool WHOLE, bool POST>
+void launch_backward(const NormArgs &a, unsigned grid, hipStream_t s)
+{
+    // sums nobody wants are left out where registers are short
+    const bool bias = a.part_b || a.part_pb;
+    if (CH > 1 && !bias)
+        hipLaunchKernelGGL((dense_norm_backward_kernel<T, TPR, VEC, CH, WHOLE, POST, CH == 1>), dim3(grid), dim3(group_threads(TPR)), 0, s, a);
+    else
+        hipLaunchKernelGGL((dense_norm_backward_kernel<T, TPR, VEC, CH, WHOLE, POST, true>), dim3(grid), dim3(group_threads(TPR)), 0, s, a);
+}
+template <class T, int TPR, int VEC, int CH, bool WHOLE>
 void launch_backward(const NormArgs &a, unsigned grid, hipStream_t s)
 {
     if (a.post_weight)
-        hipLaunchKernelGGL((dense_norm_backward_kernel<T, TPR, VEC, CH, true>), dim3(grid), dim3(group_threads(TPR)), 0, s, a);
+        launch_backward<T, TPR, VEC, CH, WHOLE, true>(a, grid, s);
     else
-        hipLaunchKernelGGL((dense_norm_backward_kernel<T, TPR, VEC, CH, false>), dim3(grid), dim3(group_threads(TPR)), 0, s, a);
+        launch_backward<T, TPR, VEC, CH, WHOLE, false>(a, grid, s);
 }
 
-// The variant is the narrowest that holds the row: 4, 8 or 16 elements a thread.
+// The narrowest variant that holds the row: 4 or 8 elements a thread (16 in the last two).  WHOLE: no thread's elements cross
+// the row's end.
 #define NORM_DISPATCH(CALL)                              \
     if (a.width <= 256) { CALL(64, 4, 1); }              \
     else if (a.width <= 512) { CALL(64, 8, 1); }         \
-    else if (a.width <= 1024) { CALL(64, 8, 2); }        \
+    else if (a.width <= 1024) { CALL(128, 8, 1); }       \
     else if (a.width <= 2048) { CALL(256, 8, 1); }       \
-    else if (a.width <= 4096) { CALL(256, 8, 2); }       \
+    else if (a.width <= 4096) { CALL(512, 8, 1); }       \
     else if (a.width <= 8192) { CALL(512, 8, 2); }       \
     else { CALL(1024, 8, 2); }
 
 template <class T>
 void dispatch_forward(const NormArgs &a, hipStream_t s)
 {
-#define CALL(TPR, VEC, CH) launch_forward<T, TPR, VEC, CH>(a, s)
+#define CALL(TPR, VEC, CH) a.width % VEC ? launch_forward<T, TPR, VEC, CH, false>(a, s) : launch_forward<T, TPR, VEC, CH, true>(a, s)
     NORM_DISPATCH(CALL)
 #undef CALL
 }
@@ -458,7 +533,7 @@ void dispatch_forward(const NormArgs &a, hipStream_t s)
 template <class T>
 void dispatch_backward(const NormArgs &a, unsigned grid, hipStream_t s)
 {
-#define CALL(TPR, VEC, CH) launch_backward<T, TPR, VEC, CH>(a, grid, s)
+#define CALL(TPR, VEC, CH) a.width % VEC ? launch_backward<T, TPR, VEC, CH, false>(a, grid, s) : launch_backward<T, TPR, VEC, CH, true>(a, grid, s)
     NORM_DISPATCH(CALL)
 #undef CALL
 }
@@ -549,7 +624,7 @@ hipError_t dn_launch_norm_backward(const opus_dense_norm_t &in, const DnDrop &dr
     groups = groups < 65535 ? groups : 65535;
 
     const unsigned grid = (unsigned)p.workgroups;
-    const dim3 rgrid((unsigned)dn_ceil(in.width, 32), (unsigned)groups, (unsigned)n);
+    const dim3 rgrid((unsigned)dn_ceil(in.width, 16), (unsigned)groups, (unsigned)n);
     const hipError_t stale = hipPeekAtLastError();
     if (in.type == OPUS_DENSE_F32) {
         if (grid) dispatch_backward<float>(a, grid, s);

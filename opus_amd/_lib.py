@@ -98,7 +98,7 @@ class DenseNorm(ctypes.Structure):
                 ("width", ctypes.c_longlong), ("gate_rows", ctypes.c_longlong), ("eps", ctypes.c_float),
                 ("scale", ctypes.c_float), ("x", ctypes.c_void_p), ("block", ctypes.c_void_p),
                 ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("post_weight", ctypes.c_void_p),
-                ("post_bias", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("dropout", ctypes.POINTER(DenseDropout))]
+                ("post_bias", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("dropout", ctypes.c_void_p)]
 
 
 class DenseNormGrads(ctypes.Structure):

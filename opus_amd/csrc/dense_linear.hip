@@ -471,6 +471,71 @@ __global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g)
     finish<T, true>(g.e, v, bias, row * g.J + col, row, col, n, (int)g.J, seed);
 }
 
+// The product for up to 16 rows of x (single tokens), bound by reading W once: 16 columns of y a workgroup, r dealt to
+// its waves.  W's rows are the matrix instruction's A operand and x's its B, both straight from memory in 16-byte
+// pieces, eight steps of r at a time; the waves' shares meet in LDS, then the epilogue.  One launch, where tiles would
+// need a second one to add the shares of r.
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(f32x4 a, f32x4 b, f32x4 c)
+{
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+}
+
+constexpr int FEW_ROWS = 16;
+
+template <class T, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) dense_few_rows_kernel(const T *x, const T *w, int M, long long N, long long K, Epilogue e)
+{
+    constexpr int PIECE = Elem<T>::PIECE, STEP = 4 * PIECE, AHEAD = 8;
+    __shared__ __align__(16) float lds[WAVES][16][20];               // [wave][row of x][column], padded
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long n0 = (long long)blockIdx.x * 16;
+    const int r = lane & 15;
+    const T *pw = w + min(n0 + r, N - 1) * K + (lane >> 4) * PIECE;  // (columns beyond N are never stored)
+    const T *px = x + (long long)min(r, M - 1) * K + (lane >> 4) * PIECE;
+    const long long each = (K + STEP * WAVES - 1) / (STEP * WAVES) * STEP;
+    const long long k0 = wave * each, k1 = min(k0 + each, K);
+    f32x4 acc = 0.f;
+    long long k = k0;
+    typename DnVec<T, PIECE>::type a[AHEAD], b[AHEAD];
+    for (; k + AHEAD * STEP <= k1; k += AHEAD * STEP) {
+#pragma unroll
+        for (int t = 0; t < AHEAD; ++t) {
+            a[t] = dn_load<PIECE>(pw + k + t * STEP);
+            b[t] = dn_load<PIECE>(px + k + t * STEP);
+        }
+#pragma unroll
+        for (int t = 0; t < AHEAD; ++t)
+            acc = mma16(a[t], b[t], acc);
+    }
+    for (; k < k1; k += STEP) {
+        const int left = (int)min(k1 - k - (lane >> 4) * PIECE, (long long)PIECE), row = (int)min(K, (long long)PIECE);
+        acc = mma16(dn_load_raw<PIECE>(pw + k, left, row), dn_load_raw<PIECE>(px + k, left, row), acc);
+    }
+    // lane: row of x lane % 16, columns 4 (lane / 16) ..
+    *reinterpret_cast<f32x4 *>(&lds[wave][r][(lane >> 4) * 4]) = acc;
+    __syncthreads();
+    const int m = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8;
+    const long long col = n0 + c;
+    const int n = (int)min(8ll, N - col);
+    if (m < M && n > 0) {
+        dn_floats<8> v = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < WAVES; ++s) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(&lds[s][m][c]), hi = *reinterpret_cast<const f32x4 *>(&lds[s][m][c + 4]);
+            v += (dn_floats<8>)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        dn_floats<8> bias = 0.f;
+        if (e.bias)
+            bias = dn_load_n<8>(static_cast<const T *>(e.bias) + col, n, (int)N);
+        finish<T, true>(e, v, bias, (uint64_t)m * N + col, m, (uint32_t)col, n, (int)N, dn_seed(e.drop));
+    }
+}
+
 // dbias from the shares of the column sums: 16 columns a workgroup, 16 lanes a column
 template <class T>
 __global__ void __launch_bounds__(256) dense_colsum_join_kernel(const float *part, int parts, long long n, T *out)
@@ -550,15 +615,22 @@ Plan plan(int type, long long I, long long J, long long R)
         return p;
     p.steps = (int)dn_ceil(R, type == OPUS_DENSE_F32 ? 32 : 64);
     p.pitch = dn_ceil(J, 8) * 8;
+    const int most = p.steps / 2 < 64 ? p.steps / 2 : 64;
+    const bool fp32 = type == OPUS_DENSE_F32;
     double best = 0;
     for (int k = 0; k < 3; ++k) {
         const TileKind &t = TILES[k];
         const long long tiles = dn_ceil(I, t.i) * dn_ceil(J, t.j);
-        const int most = p.steps / 2 < 64 ? p.steps / 2 : 64;
-        for (int n = 1; n == 1 || n <= most; ++n) {
-            const long long each = dn_ceil(p.steps, n), blocks = tiles * n, a_cu = dn_ceil(blocks, CUS);
-            const long long together = a_cu < t.per_cu ? a_cu : t.per_cu, turns = dn_ceil(a_cu, together);
-            const double step = (double)together * (type == OPUS_DENSE_F32 ? t.cost32 : t.cost16);
+        // no cut, and the cuts that give every CU 1, 2, ... workgroups, up to two turns
+        for (int m = 0; m <= 2 * t.per_cu; ++m) {
+            const long long cut = m * CUS / tiles;
+            const int n = m == 0 ? 1 : (int)(cut < most ? cut : most);
+            if (m > 0 && n < 2)
+                continue;
+            const int each = (p.steps + n - 1) / n;
+            const double a_cu = (double)((tiles * n + CUS - 1) / CUS);
+            const double together = a_cu < t.per_cu ? a_cu : t.per_cu, turns = __builtin_ceil(a_cu / together);
+            const double step = together * (fp32 ? t.cost32 : t.cost16);
             double cost = turns * (each * (step > ARRIVE ? step : ARRIVE) + START_END);
             if (n > 1)
                 cost += JOIN + 8.0 * n * I * p.pitch / JOIN_BYTES;
@@ -567,7 +639,7 @@ Plan plan(int type, long long I, long long J, long long R)
                 p.tile = k;
                 p.splits = n;
             }
-            if (blocks >= 4 * CUS * t.per_cu)
+            if (n == most)
                 break;
         }
     }
@@ -576,8 +648,8 @@ Plan plan(int type, long long I, long long J, long long R)
     p.tiles_j = (int)dn_ceil(J, t.j);
     p.steps_per_split = (int)dn_ceil(p.steps > 0 ? p.steps : 1, p.splits);
     p.splits = p.steps > 0 ? (int)dn_ceil(p.steps, p.steps_per_split) : 1;
-    const int most = p.splits < 8 ? 8 / p.splits : 1;
-    p.sharers = (p.tiles_j < most ? p.tiles_j : most) * t.waves_j;
+    const int share = p.splits < 8 ? 8 / p.splits : 1;
+    p.sharers = (p.tiles_j < share ? p.tiles_j : share) * t.waves_j;
     p.bytes = p.splits > 1 ? (size_t)p.splits * I * p.pitch * sizeof(float) : 0;
     return p;
 }
@@ -669,7 +741,25 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
 
 size_t dn_linear_forward_workspace(int type, long long M, long long N, long long K)
 {
-    return M > 0 && N > 0 ? plan(type, M, N, K).bytes : 0;
+    return M > FEW_ROWS && N > 0 ? plan(type, M, N, K).bytes : 0;
+}
+
+template <class T>
+static hipError_t forward(int type, const void *x, const void *w, long long M, long long N, long long K, const Epilogue &e,
+                          float *workspace, hipStream_t s)
+{
+    if (M > FEW_ROWS)
+        return gemm<T, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s);
+    if (dn_ceil(N, 16) * 256 > 0xFFFFFFFFll)
+        return hipErrorInvalidValue;
+    const dim3 grid((unsigned)dn_ceil(N, 16));
+    const T *tx = static_cast<const T *>(x), *tw = static_cast<const T *>(w);
+    // sixteen waves where four would leave each a long run of r, and there are too few columns to fill the chip
+    if (N <= 16 * 2 * CUS && K >= 64 * Elem<T>::STEP)
+        hipLaunchKernelGGL((dense_few_rows_kernel<T, 16>), grid, dim3(1024), 0, s, tx, tw, (int)M, N, K, e);
+    else
+        hipLaunchKernelGGL((dense_few_rows_kernel<T, 4>), grid, dim3(256), 0, s, tx, tw, (int)M, N, K, e);
+    return hipSuccess;
 }
 
 hipError_t dn_launch_linear_forward(int type, const void *x, const void *w, const void *bias, const void *residual,
@@ -680,9 +770,9 @@ hipError_t dn_launch_linear_forward(int type, const void *x, const void *w, cons
         return hipSuccess;
     const Epilogue e = {bias, residual, y, z, act, drop};
     const hipError_t stale = hipPeekAtLastError();
-    const hipError_t r = type == OPUS_DENSE_F32 ? gemm<float, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s)
-                       : type == OPUS_DENSE_BF16 ? gemm<dn_bf16, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s)
-                                                 : gemm<dn_f16, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s);
+    const hipError_t r = type == OPUS_DENSE_F32 ? forward<float>(type, x, w, M, N, K, e, workspace, s)
+                       : type == OPUS_DENSE_BF16 ? forward<dn_bf16>(type, x, w, M, N, K, e, workspace, s)
+                                                 : forward<dn_f16>(type, x, w, M, N, K, e, workspace, s);
     return r != hipSuccess ? r : msmv_launch_status(stale);
 }
 

@@ -24,6 +24,7 @@ when that tensor is changed between replays.  It must not change between a forwa
 dropout of a step an ``offset`` (0 .. 2**32 - 1) of its own.
 """
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -36,21 +37,21 @@ _TYPES = {torch.float32: _lib.DENSE_F32, torch.bfloat16: _lib.DENSE_BF16, torch.
 # ------------------------------------------------------------------------------------------------
 # arguments
 # ------------------------------------------------------------------------------------------------
-def _check(what, x, others):
-    """One type, one GPU; ``others`` maps names to tensors or None."""
+def _check(what, x, names, others):
+    """One type, one GPU; ``others`` are tensors or None, ``names`` what they are called."""
     if not x.is_cuda:
         raise RuntimeError(f"{what}: expected CUDA tensors")
-    if x.dtype not in _TYPES:
-        raise RuntimeError(f"{what}: expected float32, bfloat16 or float16 tensors, got {x.dtype}")
+    dtype, device = x.dtype, x.device
+    if dtype not in _TYPES:
+        raise RuntimeError(f"{what}: expected float32, bfloat16 or float16 tensors, got {dtype}")
     if x.dim() < 1:
         raise RuntimeError(f"{what}: expected a tensor of at least one dimension")
-    for name, t in others:
-        if t is None:
-            continue
-        if t.dtype != x.dtype:
-            raise RuntimeError(f"{what}: {name} is {t.dtype}, expected {x.dtype}")
-        if t.device != x.device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, expected {x.device}")
+    for i, t in enumerate(others):
+        if t is not None:
+            if t.dtype != dtype:
+                raise RuntimeError(f"{what}: {names[i]} is {t.dtype}, expected {dtype}")
+            if t.device != device:
+                raise RuntimeError(f"{what}: {names[i]} is on {t.device}, expected {device}")
 
 
 def _threshold(what, p, seed, offset, device):
@@ -78,18 +79,28 @@ def _drop_struct(threshold, seed, offset):
     return _lib.DenseDropout(threshold, offset, seed & (2 ** 64 - 1), None)
 
 
+def _seed_tensor(threshold, seed):
+    """The seed as what autograd keeps an eye on (None for a number): changed in place before the backward, it would
+    give another mask there."""
+    return seed if threshold and isinstance(seed, torch.Tensor) else None
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+# the current stream's handle: what torch.cuda.current_stream(index).cuda_stream gives, without making a Stream object
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _run(what, fn, device, *args):
     """Calls a C entry, whose last argument is the stream, with ``device`` current."""
     index = device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, _stream(index))
     if rc != 0:
         _lib.check_dense(rc, what)
 
@@ -98,65 +109,89 @@ def _contiguous(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _wants_grad(tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _first_order(backward):
+    """``once_differentiable``, entered only where a graph of the backward is asked for."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return staticmethod(run)
+
+
+# sizes alone decide these
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(kind, M, N, K):
+    return _lib.load().opus_dense_linear_workspace_bytes(kind, M, N, K)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_backward_workspace(kind, M, N, K):
+    return _lib.load().opus_dense_linear_backward_workspace_bytes(kind, M, N, K)
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_backward_workspace(kind, rows, width, gate_rows):
+    return _lib.load().opus_dense_norm_backward_workspace_bytes(kind, rows, width, gate_rows)
 
 
 # ------------------------------------------------------------------------------------------------
 # linear
 # ------------------------------------------------------------------------------------------------
-def _linear_forward(x, weight, bias, residual, activation, threshold, seed, offset, want_z):
-    lib = _lib.load()
+def _linear_forward(x, weight, bias, residual, activation, drop, want_z):
     N, K = weight.shape
-    shape = x.shape[:-1] + (N,)
     x, weight, bias, residual = _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual)
-    M = x.numel() // K if K else shape.numel() // max(N, 1)
-    kind = _TYPES[x.dtype]
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(shape, dtype=x.dtype, device=x.device) if want_z else None
-    need = lib.opus_dense_linear_workspace_bytes(kind, M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _run("linear", lib.opus_dense_linear_forward, x.device, kind, x.data_ptr(), weight.data_ptr(), _ptr(bias),
-         _ptr(residual), M, N, K, activation, _drop_struct(threshold, seed, offset), y.data_ptr(), _ptr(z), _ptr(ws),
-         need)
+    kind, device = _TYPES[x.dtype], x.device
+    y = x.new_empty(x.shape[:-1] + (N,))
+    M = x.numel() // K if K else y.numel() // max(N, 1)
+    z = torch.empty_like(y) if want_z else None
+    need = _linear_workspace(kind, M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _run("linear", _lib.load().opus_dense_linear_forward, device, kind, x.data_ptr(), weight.data_ptr(), _ptr(bias),
+         _ptr(residual), M, N, K, activation, drop, y.data_ptr(), _ptr(z), _ptr(ws), need)
     return y, z
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, threshold, seed, offset):
-        y, z = _linear_forward(x, weight, bias, residual, activation, threshold, seed, offset, activation != 0)
-        seed_tensor = seed if isinstance(seed, torch.Tensor) and threshold else None
-        ctx.save_for_backward(x, weight, z, seed_tensor)
-        ctx.settings = activation, threshold, None if seed_tensor is not None else seed, offset
+        drop = _drop_struct(threshold, seed, offset)
+        y, z = _linear_forward(x, weight, bias, residual, activation, drop, activation != 0)
+        ctx.save_for_backward(x, weight, z, _seed_tensor(threshold, seed))
+        ctx.settings = activation, drop
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
-        x, weight, z, seed_tensor = ctx.saved_tensors
-        activation, threshold, seed, offset = ctx.settings
+        x, weight, z, _ = ctx.saved_tensors
+        activation, drop = ctx.settings
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
-            lib = _lib.load()
             N, K = weight.shape
-            shape, kind, device = x.shape, _TYPES[x.dtype], x.device
-            x, weight, g = _contiguous(x), _contiguous(weight), _contiguous(dy)
+            kind, device = _TYPES[x.dtype], x.device
             M = x.numel() // K if K else dy.numel() // max(N, 1)
+            x, weight, g = _contiguous(x), _contiguous(weight), _contiguous(dy)
             if need_x:
-                dx = torch.empty(shape, dtype=x.dtype, device=device)
+                dx = torch.empty_like(x)
             if need_w:
-                dw = torch.empty((N, K), dtype=x.dtype, device=device)
+                dw = torch.empty_like(weight)
             if need_b:
-                db = torch.empty((N,), dtype=x.dtype, device=device)
-            dz = torch.empty_like(g) if activation or threshold else None
-            need = lib.opus_dense_linear_backward_workspace_bytes(kind, M, N, K)
+                db = weight.new_empty(N)
+            dz = torch.empty_like(g) if activation or drop is not None else None
+            need = _linear_backward_workspace(kind, M, N, K)
             ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-            _run("linear backward", lib.opus_dense_linear_backward, device, kind, g.data_ptr(), x.data_ptr(),
-                 weight.data_ptr(), _ptr(z), M, N, K, activation,
-                 _drop_struct(threshold, seed if seed_tensor is None else seed_tensor, offset), _ptr(dz), _ptr(dx),
-                 _ptr(dw), _ptr(db), _ptr(ws), need)
+            _run("linear backward", _lib.load().opus_dense_linear_backward, device, kind, g.data_ptr(), x.data_ptr(),
+                 weight.data_ptr(), _ptr(z), M, N, K, activation, drop, _ptr(dz), _ptr(dx), _ptr(dw), _ptr(db),
+                 _ptr(ws), need)
         return dx, dw, db, dy if need_r else None, None, None, None, None
 
 
@@ -168,20 +203,21 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout_p=0.0
     Gradients flow to x, weight, bias and residual.  With an activation the backward needs x W^T + bias, which the
     forward then stores in the tensors' type (only where a gradient is wanted); d act(x W^T + bias) is rounded to that
     type too before the two products of the backward."""
-    _check("linear", x, (("weight", weight), ("bias", bias), ("residual", residual)))
-    if weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
-        raise RuntimeError(f"linear: weight {list(weight.shape)} does not fit x {list(x.shape)}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise RuntimeError(f"linear: bias {list(bias.shape)} does not fit weight {list(weight.shape)}")
-    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
+    _check("linear", x, ("weight", "bias", "residual"), (weight, bias, residual))
+    shape, w_shape = x.shape, weight.shape
+    if len(w_shape) != 2 or w_shape[1] != shape[-1]:
+        raise RuntimeError(f"linear: weight {list(w_shape)} does not fit x {list(shape)}")
+    if bias is not None and bias.shape != w_shape[:1]:
+        raise RuntimeError(f"linear: bias {list(bias.shape)} does not fit weight {list(w_shape)}")
+    if residual is not None and residual.shape != shape[:-1] + w_shape[:1]:
         raise RuntimeError(f"linear: residual {list(residual.shape)} is not of the output's shape")
-    if activation not in _lib.DENSE_ACTIVATIONS:
+    code = _lib.DENSE_ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"linear: activation has to be one of {sorted(_lib.DENSE_ACTIVATIONS)}, got {activation!r}")
-    threshold = _threshold("linear", dropout_p, seed, offset, x.device)
-    code = _lib.DENSE_ACTIVATIONS[activation]
-    if _wants_grad(x, weight, bias, residual):
+    threshold = _threshold("linear", dropout_p, seed, offset, x.device) if dropout_p != 0.0 else 0
+    if _wants_grad((x, weight, bias, residual)):
         return _Linear.apply(x, weight, bias, residual, code, threshold, seed, offset)
-    return _linear_forward(x, weight, bias, residual, code, threshold, seed, offset, False)[0]
+    return _linear_forward(x, weight, bias, residual, code, _drop_struct(threshold, seed, offset), False)[0]
 
 
 # ------------------------------------------------------------------------------------------------
@@ -191,58 +227,55 @@ def _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop):
     x, block, weight, bias, post_weight, post_bias, gate = tensors
     return _lib.DenseNorm(_TYPES[x.dtype], kind, rows, x.shape[-1], gate_rows, eps, scale, x.data_ptr(),
                           block.data_ptr(), _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
-                          ctypes.pointer(drop) if drop is not None else None)
+                          None if drop is None else ctypes.addressof(drop))
 
 
-def _norm_forward(tensors, kind, gate_rows, eps, scale, threshold, seed, offset, want_stream, want_stats):
-    lib = _lib.load()
+def _norm_forward(tensors, kind, gate_rows, eps, scale, drop, want_stream, want_stats):
     tensors = [_contiguous(t) for t in tensors]
     x = tensors[0]
     rows = x.numel() // x.shape[-1]
     y = torch.empty_like(x)
     stream = torch.empty_like(x) if want_stream else None
     stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
-    args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, _drop_struct(threshold, seed, offset))
-    _run("residual_norm", lib.opus_dense_norm_forward, x.device, args, y.data_ptr(), _ptr(stream), _ptr(stats))
+    args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop)
+    _run("residual_norm", _lib.load().opus_dense_norm_forward, x.device, args, y.data_ptr(), _ptr(stream), _ptr(stats))
     return y, stream, stats
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, block, weight, bias, post_weight, post_bias, gate, kind, gate_rows, eps, scale, threshold, seed,
-                offset, want_stream):
+    def forward(ctx, x, block, weight, bias, post_weight, post_bias, gate, settings):
+        kind, gate_rows, eps, scale, threshold, seed, offset, want_stream = settings
         tensors = (x, block, weight, bias, post_weight, post_bias, gate)
-        y, stream, stats = _norm_forward(tensors, kind, gate_rows, eps, scale, threshold, seed, offset, want_stream,
-                                         True)
-        seed_tensor = seed if isinstance(seed, torch.Tensor) and threshold else None
-        ctx.save_for_backward(*tensors, stats, seed_tensor)
-        ctx.settings = kind, gate_rows, eps, scale, threshold, None if seed_tensor is not None else seed, offset
+        drop = _drop_struct(threshold, seed, offset)
+        y, stream, stats = _norm_forward(tensors, kind, gate_rows, eps, scale, drop, want_stream, True)
+        ctx.save_for_backward(*tensors, stats, _seed_tensor(threshold, seed))
+        ctx.settings = kind, gate_rows, eps, scale, drop
         ctx.set_materialize_grads(False)
         return (y, stream) if want_stream else y
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dstream=None):
-        *tensors, stats, seed_tensor = ctx.saved_tensors
-        kind, gate_rows, eps, scale, threshold, seed, offset = ctx.settings
-        none = (None,) * 8
         if dy is None and dstream is None:
-            return (None,) * 7 + none
-        lib = _lib.load()
-        grads = [torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and need else None
-                 for t, need in zip(tensors, ctx.needs_input_grad)]
-        tensors = [_contiguous(t) for t in tensors]
+            return (None,) * 8
+        saved = ctx.saved_tensors
+        kind, gate_rows, eps, scale, drop = ctx.settings
+        tensors, stats = [_contiguous(t) for t in saved[:7]], saved[7]
+        grads = [torch.empty_like(t) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
         x = tensors[0]
-        rows, width = x.numel() // x.shape[-1], x.shape[-1]
+        width = x.shape[-1]
+        rows = x.numel() // width
         dy, dstream = _contiguous(dy), _contiguous(dstream)
-        drop = _drop_struct(threshold, seed if seed_tensor is None else seed_tensor, offset)
         args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop)
-        need = lib.opus_dense_norm_backward_workspace_bytes(args.type, rows, width,
-                                                            gate_rows if tensors[6] is not None else 0)
+        need = _norm_backward_workspace(args.type, rows, width, gate_rows)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        _run("residual_norm backward", lib.opus_dense_norm_backward, x.device, args, _ptr(dy), _ptr(dstream),
-             stats.data_ptr(), _lib.DenseNormGrads(*[_ptr(g) for g in grads]), _ptr(ws), need)
-        return (*grads, *none)
+        _run("residual_norm backward", _lib.load().opus_dense_norm_backward, x.device, args, _ptr(dy), _ptr(dstream),
+             stats.data_ptr(), _lib.DenseNormGrads(*[None if g is None else g.data_ptr() for g in grads]), _ptr(ws),
+             need)
+        return (*grads, None)
+
+
+_NORM_NAMES = ("block", "weight", "bias", "post_weight", "post_bias", "gate")
 
 
 def _gate_rows(x, gate):
@@ -281,71 +314,68 @@ def residual_norm(x, block, weight=None, bias=None, kind="layer", eps=1e-5, post
     Returns y, or (y, r) with ``return_stream``.  y is computed from the unrounded r.  Gradients flow to all tensors,
     from either result; the backward computes r again from x and block, so that only two statistics for each norm
     and row are kept."""
-    _check("residual_norm", x, (("block", block), ("weight", weight), ("bias", bias), ("post_weight", post_weight),
-                                ("post_bias", post_bias), ("gate", gate)))
-    width = x.shape[-1]
-    if block.shape != x.shape:
-        raise RuntimeError(f"residual_norm: block {list(block.shape)} is not of x's shape {list(x.shape)}")
+    tensors = (x, block, weight, bias, post_weight, post_bias, gate)
+    _check("residual_norm", x, _NORM_NAMES, tensors[1:])
+    shape = x.shape
+    width = shape[-1]
+    if block.shape != shape:
+        raise RuntimeError(f"residual_norm: block {list(block.shape)} is not of x's shape {list(shape)}")
     if not 1 <= width <= _lib.DENSE_MAX_WIDTH:
         raise RuntimeError(f"residual_norm: width has to be in [1, {_lib.DENSE_MAX_WIDTH}], got {width}")
-    for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
-        if t is not None and t.shape != (width,):
-            raise RuntimeError(f"residual_norm: {name} {list(t.shape)} has to be [{width}]")
+    for i in range(2, 6):
+        t = tensors[i]
+        if t is not None and (t.dim() != 1 or t.shape[0] != width):
+            raise RuntimeError(f"residual_norm: {_NORM_NAMES[i - 1]} {list(t.shape)} has to be [{width}]")
     if post_bias is not None and post_weight is None:
         raise RuntimeError("residual_norm: post_bias without post_weight")
-    if kind not in _lib.DENSE_NORMS:
+    code = _lib.DENSE_NORMS.get(kind)
+    if code is None:
         raise ValueError(f"residual_norm: kind has to be one of {sorted(_lib.DENSE_NORMS)}, got {kind!r}")
     gate_rows = 0 if gate is None else _gate_rows(x, gate)
-    threshold = _threshold("residual_norm", dropout_p, seed, offset, x.device)
-    tensors = (x, block, weight, bias, post_weight, post_bias, gate)
-    code = _lib.DENSE_NORMS[kind]
-    if _wants_grad(*tensors):
-        return _ResidualNorm.apply(*tensors, code, gate_rows, eps, residual_scale, threshold, seed, offset,
-                                   return_stream)
-    y, stream, _ = _norm_forward(tensors, code, gate_rows, eps, residual_scale, threshold, seed, offset, return_stream,
-                                 False)
+    threshold = _threshold("residual_norm", dropout_p, seed, offset, x.device) if dropout_p != 0.0 else 0
+    if _wants_grad(tensors):
+        return _ResidualNorm.apply(*tensors, (code, gate_rows, eps, residual_scale, threshold, seed, offset,
+                                              return_stream))
+    y, stream, _ = _norm_forward(tensors, code, gate_rows, eps, residual_scale, _drop_struct(threshold, seed, offset),
+                                 return_stream, False)
     return (y, stream) if return_stream else y
 
 
 # ------------------------------------------------------------------------------------------------
 # dropout
 # ------------------------------------------------------------------------------------------------
-def _dropout(x, residual, threshold, seed, offset):
-    lib = _lib.load()
+def _dropout(x, residual, drop):
     x, residual = _contiguous(x), _contiguous(residual)
     cols = x.shape[-1]
     y = torch.empty_like(x)
-    _run("dropout", lib.opus_dense_dropout, x.device, _TYPES[x.dtype], x.data_ptr(), _ptr(residual),
-         x.numel() // max(cols, 1), cols, _drop_struct(threshold, seed, offset), y.data_ptr())
+    _run("dropout", _lib.load().opus_dense_dropout, x.device, _TYPES[x.dtype], x.data_ptr(), _ptr(residual),
+         x.numel() // max(cols, 1), cols, drop, y.data_ptr())
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, threshold, seed, offset):
-        seed_tensor = seed if isinstance(seed, torch.Tensor) and threshold else None
-        ctx.save_for_backward(seed_tensor)
-        ctx.settings = threshold, None if seed_tensor is not None else seed, offset
-        return _dropout(x, residual, threshold, seed, offset)
+        ctx.drop = _drop_struct(threshold, seed, offset)
+        watched = _seed_tensor(threshold, seed)
+        if watched is not None:
+            ctx.save_for_backward(watched)
+        return _dropout(x, residual, ctx.drop)
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
-        seed_tensor, = ctx.saved_tensors
-        threshold, seed, offset = ctx.settings
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _dropout(dy, None, threshold, seed if seed_tensor is None else seed_tensor, offset)
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        ctx.saved_tensors                       # (a seed tensor that was changed since is an error)
+        need_x, need_r = ctx.needs_input_grad[:2]
+        return _dropout(dy, None, ctx.drop) if need_x else None, dy if need_r else None, None, None, None
 
 
 def dropout(x, p, seed, offset=0, residual=None):
     """``residual + D(x)``: x [..., columns], residual of x's shape or None.  See the module's text for ``D``.
     Gradients flow to x and residual."""
-    _check("dropout", x, (("residual", residual),))
+    _check("dropout", x, ("residual",), (residual,))
     if residual is not None and residual.shape != x.shape:
         raise RuntimeError(f"dropout: residual {list(residual.shape)} is not of x's shape {list(x.shape)}")
     threshold = _threshold("dropout", p, seed, offset, x.device)
-    if _wants_grad(x, residual):
+    if _wants_grad((x, residual)):
         return _Dropout.apply(x, residual, threshold, seed, offset)
-    return _dropout(x, residual, threshold, seed, offset)
+    return _dropout(x, residual, _drop_struct(threshold, seed, offset))

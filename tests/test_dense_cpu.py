@@ -54,10 +54,10 @@ def test_linear_arguments(lib):
     assert forward(drop=_lib.DenseDropout(65537, 0, 0, None)) == -6
     assert forward(drop=_lib.DenseDropout(1, 0, 0, 4100)) == -3        # seed address not a multiple of eight
     assert forward(M=0) == 0 and forward(N=0) == 0
-    need = lib.opus_dense_linear_workspace_bytes(0, 4, 8, 1 << 16)
-    assert need > 0 and forward(K=1 << 16) == -5
-    assert forward(K=1 << 16, ws=SOME, nws=need - 1) == -5
-    assert forward(K=1 << 16, ws=ctypes.c_void_p(4100), nws=need) == -5
+    need = lib.opus_dense_linear_workspace_bytes(0, 64, 8, 1 << 16)
+    assert need > 0 and forward(M=64, K=1 << 16) == -5
+    assert forward(M=64, K=1 << 16, ws=SOME, nws=need - 1) == -5
+    assert forward(M=64, K=1 << 16, ws=ctypes.c_void_p(4100), nws=need) == -5
 
     def backward(dy=SOME, x=SOME, w=SOME, z=SOME, M=4, N=8, K=16, act=0, drop=None, dz=SOME, dx=SOME, dw=SOME, db=SOME,
                  ws=NULL, nws=0):
@@ -76,7 +76,7 @@ def test_norm_and_dropout_arguments(lib):
 
     def struct(type=0, kind=0, rows=4, width=8, gate_rows=0, x=SOME, block=SOME, gate=None, drop=None):
         return _lib.DenseNorm(type, kind, rows, width, gate_rows, 1e-5, 1.0, x.value, block.value, None, None, None, None,
-                              gate, ctypes.pointer(drop) if drop else None)
+                              gate, ctypes.addressof(drop) if drop else None)
 
     def forward(y=SOME, stats=NULL, **kw):
         return lib.opus_dense_norm_forward(struct(**kw), y, NULL, stats, None)

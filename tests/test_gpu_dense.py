@@ -128,6 +128,16 @@ def test_linear_activations_with_dropout(od, dtype, name):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_linear_few_rows(od, dtype):
+    """Up to 16 rows of x go through a kernel of their own: both its widths, whole and odd lengths, every row count."""
+    for i, M in enumerate(range(1, 18)):
+        run_linear(od, 100 + i, TYPES[dtype], M, 64 * (i + 1) + (0, 1, 8)[i % 3], 33 + 17 * i, name=ACTS[i % 5], p=0.2, train=i % 4 == 0)
+    run_linear(od, 120, TYPES[dtype], 1, 8200, 4096, name="silu", train=False)
+    run_linear(od, 121, TYPES[dtype], 3, 4099, 57, train=False)
+    run_linear(od, 122, TYPES[dtype], 16, 2048, 9001, train=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
 def test_linear_many_tiles(od, dtype):
     """Whole and partial tiles of the wide variants, more than one band of tile rows, all three products."""
     run_linear(od, 60, TYPES[dtype], 1100, 192, 1300, bias=True, residual=False)

@@ -75,8 +75,9 @@ struct GemmArgs {
     int tiles_i, tiles_j, splits, steps, steps_per_split;       // steps: tiles of 128 bytes along r
     float *partial;              // [splits][I][pitch], where splits > 1
     long long pitch;
-    float *colsum;               // [splits * sharers][I]: sum over r of A(i, r), NULL: not wanted
-    int sharers;                 // tiles of a row of tiles that share the column sums' work, times the waves side by side
+    float *colsum;               // [splits * sharers][I]: shares of the sums over r of A(i, r) ..
+    void *colsum_out;            // .. which belong here (at once, where there is one share); NULL: not wanted
+    int sharers;                 // tiles of a row of tiles that share the sums' work
     Epilogue e;
 };
 
@@ -309,10 +310,9 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
 #pragma unroll
     for (int i = 0; i < MI; ++i)
         sum[i] = 0.f;
-    // The sums of A's rows: of a row of tiles the first `share` take turns at the steps of r, and of the waves that hold
+    // The sums of A's rows: of a row of tiles the first `sharers` take turns at the steps of r, and of the waves that hold
     // the same rows each takes its k-groups of a step.
-    const int share = g.sharers / WJ;
-    const bool summing = !ARC && g.colsum && tj < share;
+    const bool summing = !ARC && g.colsum_out && tj < g.sharers;
 
     typename DnVec<T, Elem<T>::PIECE>::type fa[2][MI], fb[2][MJ];
     const auto load = [&](const char *from, int ks) __attribute__((always_inline)) {
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
             fetch(next);
         load(cur, 0);
         for (int s = s0; s < s1; ++s) {
-            turn_to_sum = summing && s % share == tj;
+            turn_to_sum = summing && s % g.sharers == tj;
             const bool more = s + 1 < s1, by_hand = more && s + 1 >= whole;
             if (!DIRECT && by_hand)             // under way while this tile is multiplied
                 read(s + 1);
@@ -383,13 +383,28 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
         }
     }
 
-    if (!ARC && summing)
+    if constexpr (!ARC)
+        if (summing) {                            // (uniform over the workgroup)
+            __syncthreads();
+            float *rows = reinterpret_cast<float *>(lds);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const float t = sum[i] + __shfl_xor(sum[i], 32);
-            const long long row = i0 + (wi * MI + i) * 32 + (lane & 31);
-            if (lane < 32 && row < g.I)
-                g.colsum[((long long)split * g.sharers + tj * WJ + wj) * g.I + row] = t;
+            for (int i = 0; i < MI; ++i) {
+                const float t = sum[i] + __shfl_xor(sum[i], 32);
+                if (lane < 32)
+                    rows[wj * BM + (wi * MI + i) * 32 + lane] = t;
+            }
+            __syncthreads();
+            for (int r = tid; r < BM; r += THREADS)
+                if (i0 + r < g.I) {
+                    float t = rows[r];
+#pragma unroll
+                    for (int k = 1; k < WJ; ++k)
+                        t += rows[k * BM + r];
+                    if (g.colsum)
+                        g.colsum[((long long)split * g.sharers + tj) * g.I + i0 + r] = t;
+                    else
+                        static_cast<T *>(g.colsum_out)[i0 + r] = (T)t;
+                }
         }
 
     // ---- epilogue: a wave turns 32 rows x (32 MJ, at most 64) columns at a time through its own strip
@@ -449,10 +464,38 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
     }
 }
 
-// Adds the shares of r in order and runs the epilogue; a thread takes eight columns of a row.
+// The column sums' shares added up, by 256 threads: 16 columns, 16 lanes a column.
 template <class T>
-__global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g)
+__device__ __forceinline__ void join_sums(const float *part, int parts, long long n, T *out, long long block)
 {
+    __shared__ float lds[16][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const long long i = block * 16 + x;
+    float s = 0.f;
+    if (i < n) {
+#pragma unroll 4
+        for (int k = y; k < parts; k += 16)
+            s += part[k * n + i];
+    }
+    lds[y][x] = s;
+    __syncthreads();
+    if (y == 0 && i < n) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k)
+            s += lds[k][x];
+        out[i] = (T)s;
+    }
+}
+
+// Adds the shares of r in order and runs the epilogue; a thread takes eight columns of a row.  The workgroups behind
+// those, if any, add the column sums' shares.
+template <class T>
+__global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g, unsigned blocks)
+{
+    if (blockIdx.x >= blocks) {
+        join_sums<T>(g.colsum, g.splits * g.sharers, g.I, static_cast<T *>(g.colsum_out), blockIdx.x - blocks);
+        return;
+    }
     const uint64_t seed = dn_seed(g.e.drop);
     const uint32_t units = (uint32_t)(g.pitch / 8);
     const uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x;
@@ -462,8 +505,9 @@ __global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g)
         return;
     dn_floats<8> v = 0.f;
     const float *p = g.partial + row * g.pitch + col;
-    for (int s = 0; s < g.splits; ++s, p += g.I * g.pitch)
-        v += *reinterpret_cast<const dn_floats<8> *>(p);
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s)
+        v += *reinterpret_cast<const dn_floats<8> *>(p + s * g.I * g.pitch);
     const int n = (int)min(8ll, g.J - (long long)col);
     dn_floats<8> bias = 0.f;
     if (g.e.bias)
@@ -536,27 +580,10 @@ __global__ void __launch_bounds__(WAVES * 64) dense_few_rows_kernel(const T *x, 
     }
 }
 
-// dbias from the shares of the column sums: 16 columns a workgroup, 16 lanes a column
 template <class T>
 __global__ void __launch_bounds__(256) dense_colsum_join_kernel(const float *part, int parts, long long n, T *out)
 {
-    __shared__ float lds[16][17];
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-    const long long i = (long long)blockIdx.x * 16 + x;
-    float s = 0.f;
-    if (i < n) {
-#pragma unroll 4
-        for (int k = y; k < parts; k += 16)
-            s += part[k * n + i];
-    }
-    lds[y][x] = s;
-    __syncthreads();
-    if (y == 0 && i < n) {
-#pragma unroll
-        for (int k = 1; k < 16; ++k)
-            s += lds[k][x];
-        out[i] = (T)s;
-    }
+    join_sums<T>(part, parts, n, out, blockIdx.x);
 }
 
 // Column sums of dz [M, N] by themselves (where dW is not wanted, or has no elements): 32 columns a workgroup
@@ -594,18 +621,18 @@ struct Plan {
     int sharers;                 // of the column sums
 };
 
-// The tiles a workgroup can make, rows x columns of C, the workgroups of a kind that fit a CU together (by LDS), its
-// waves side by side, and what a step of r costs one of them, in cycles, where the CU is full (16-bit types, fp32).
+// The tiles a workgroup can make, rows x columns of C, the workgroups of a kind that fit a CU together (by LDS), and what
+// a step of r costs one of them, in cycles, where the CU is full (16-bit types, fp32).
 struct TileKind {
-    int i, j, per_cu, waves_j, cost16, cost32;
+    int i, j, per_cu, cost16, cost32;
 };
-constexpr TileKind TILES[] = {{64, 64, 4, 2, 330, 1350}, {128, 128, 2, 2, 800, 4700}, {256, 256, 1, 4, 2560, 18200}};
+constexpr TileKind TILES[] = {{64, 64, 4, 330, 1350}, {128, 128, 2, 800, 4700}, {256, 256, 1, 2560, 18200}};
 
 // Which tile, and into how many shares r is cut: the cheapest by this estimate.  A CU works through its workgroups in
 // turns of as many as fit it; a step of r costs them together the cost above, and never less than the time a transfer
 // takes to arrive; a workgroup's start and end cost about as much as a few steps; shares are written, read and added by
 // a further kernel.
-constexpr double ARRIVE = 1400, START_END = 8000, JOIN = 8000, JOIN_BYTES = 2000;
+constexpr double ARRIVE = 1400, START_END = 8000, JOIN = 14000, JOIN_BYTES = 2000;
 
 Plan plan(int type, long long I, long long J, long long R)
 {
@@ -648,8 +675,9 @@ Plan plan(int type, long long I, long long J, long long R)
     p.tiles_j = (int)dn_ceil(J, t.j);
     p.steps_per_split = (int)dn_ceil(p.steps > 0 ? p.steps : 1, p.splits);
     p.splits = p.steps > 0 ? (int)dn_ceil(p.steps, p.steps_per_split) : 1;
-    const int share = p.splits < 8 ? 8 / p.splits : 1;
-    p.sharers = (p.tiles_j < share ? p.tiles_j : share) * t.waves_j;
+    // the column sums are shared where there is much of r to a tile, else one tile's work costs less than another launch
+    const int share = p.splits == 1 && p.steps >= 48 ? 8 : 1;
+    p.sharers = p.tiles_j < share ? p.tiles_j : share;
     p.bytes = p.splits > 1 ? (size_t)p.splits * I * p.pitch * sizeof(float) : 0;
     return p;
 }
@@ -668,16 +696,17 @@ void launch_tiles(const Plan &p, const GemmArgs &g, hipStream_t s)
         hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 2, 1, 1, DIRECT>), grid, dim3(256), 0, s, g);
 }
 
-// C = A B^T with an epilogue; `shares`: p.bytes of workspace.  colsum: [p.splits * p.sharers][I] fp32 or NULL.
+// C = A B^T with an epilogue; `shares`: p.bytes of workspace.  sums_out [I]: the sums over r of A(i, r), or NULL; `sums`:
+// [p.splits * p.sharers][I] of workspace for them.
 template <class T, bool ARC, bool BRC>
 hipError_t gemm(int type, const void *a, const void *b, long long I, long long J, long long R, const Epilogue &e,
-                float *shares, float *colsum, hipStream_t s)
+                float *shares, float *sums, void *sums_out, hipStream_t s)
 {
     const Plan p = plan(type, I, J, R);
     if ((long long)p.tiles_i * p.tiles_j * p.splits * 256 > 0xFFFFFFFFll)
         return hipErrorInvalidValue;
     GemmArgs g = {a, b, I, J, R, p.tiles_i, p.tiles_j, p.splits, p.steps, p.steps_per_split,
-                  p.splits > 1 ? shares : nullptr, p.pitch, colsum, p.sharers, e};
+                  p.splits > 1 ? shares : nullptr, p.pitch, p.splits * p.sharers > 1 ? sums : nullptr, sums_out, p.sharers, e};
     const int piece = Elem<T>::PIECE;
     // (a tile's pieces are addressed in 32 bits from its corner)
     const auto near = [](bool rc, long long i, long long r) { return (rc ? 256 * r : 64 * i) * sizeof(T) < (1ll << 31); };
@@ -687,11 +716,15 @@ hipError_t gemm(int type, const void *a, const void *b, long long I, long long J
         launch_tiles<T, ARC, BRC, true>(p, g, s);
     else
         launch_tiles<T, ARC, BRC, false>(p, g, s);
+    const long long sum_blocks = sums_out && g.colsum ? dn_ceil(I, 16) : 0;
     if (p.splits > 1) {
         const long long blocks = dn_ceil(I * (p.pitch / 8), 256);
-        if (blocks * 256 > 0xFFFFFFFFll)
+        if ((blocks + sum_blocks) * 256 > 0xFFFFFFFFll)
             return hipErrorInvalidValue;
-        hipLaunchKernelGGL(dense_gemm_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, g);
+        hipLaunchKernelGGL(dense_gemm_join_kernel<T>, dim3((unsigned)(blocks + sum_blocks)), dim3(256), 0, s, g, (unsigned)blocks);
+    } else if (sum_blocks) {
+        hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)sum_blocks), dim3(256), 0, s, g.colsum, p.sharers, I,
+                           static_cast<T *>(sums_out));
     }
     return hipSuccess;
 }
@@ -713,7 +746,7 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
     hipError_t e = hipSuccess;
     if (dx && M && K) {
         const Epilogue ep = {nullptr, nullptr, dx, nullptr, OPUS_DENSE_ACT_NONE, {}};
-        e = gemm<T, true, false>(type, dz, w, M, K, N, ep, ws, nullptr, s);
+        e = gemm<T, true, false>(type, dz, w, M, K, N, ep, ws, nullptr, nullptr, s);
     }
     if (e != hipSuccess)
         return e;
@@ -721,12 +754,7 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
     float *sums = ws + align256(p.bytes) / sizeof(float);
     if (dw && N && K) {
         const Epilogue ep = {nullptr, nullptr, dw, nullptr, OPUS_DENSE_ACT_NONE, {}};
-        e = gemm<T, false, false>(type, dz, x, N, K, M, ep, ws, db ? sums : nullptr, s);
-        if (e != hipSuccess)
-            return e;
-        if (db)
-            hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 16)), dim3(256), 0, s, sums,
-                               p.splits * p.sharers, N, static_cast<T *>(db));
+        e = gemm<T, false, false>(type, dz, x, N, K, M, ep, ws, sums, db, s);
     } else if (db && N) {
         const long long runs = colsum_runs(M, N), per = dn_ceil(M > 0 ? M : 1, runs);
         hipLaunchKernelGGL(dense_colsum_kernel<T>, dim3((unsigned)dn_ceil(N, 32), (unsigned)runs), dim3(256), 0, s,
@@ -749,7 +777,7 @@ static hipError_t forward(int type, const void *x, const void *w, long long M, l
                           float *workspace, hipStream_t s)
 {
     if (M > FEW_ROWS)
-        return gemm<T, true, true>(type, x, w, M, N, K, e, workspace, nullptr, s);
+        return gemm<T, true, true>(type, x, w, M, N, K, e, workspace, nullptr, nullptr, s);
     if (dn_ceil(N, 16) * 256 > 0xFFFFFFFFll)
         return hipErrorInvalidValue;
     const dim3 grid((unsigned)dn_ceil(N, 16));

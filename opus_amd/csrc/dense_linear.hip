@@ -246,22 +246,23 @@ __device__ __forceinline__ float add_up(f32x4 v, float s) { return s + ((v[0] + 
 constexpr int STRIP = 72;       // floats a row of a wave's strip in LDS: rows four apart then start 32 banks apart
 
 // WI x WJ waves, each MI x MJ blocks of 32 x 32.  DIRECT: bases and rows are 16-byte aligned.
+template <class T, int WI, int WJ, int MI, int MJ>
+constexpr int gemm_lds = (2 * (WI * MI + WJ * MJ) * 32 * 128 > WI * WJ * 32 * STRIP * 4) ? 2 * (WI * MI + WJ * MJ) * 32 * 128 : WI * WJ * 32 * STRIP * 4;
+
 template <class T, bool ARC, bool BRC, int WI, int WJ, int MI, int MJ, bool DIRECT>
-__global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
+__device__ __forceinline__ void gemm_tile(const GemmArgs &g, int id, char *lds)
 {
     constexpr int THREADS = WI * WJ * 64, BM = WI * MI * 32, BN = WJ * MJ * 32, STEP = Elem<T>::STEP;
     using TA = Tile<T, ARC, BM>;
     using TB = Tile<T, BRC, BN>;
     constexpr int STAGE = TA::BYTES + TB::BYTES;
-    constexpr int STRIPS = WI * WJ * 32 * STRIP * 4;
-    __shared__ __align__(128) char lds[2 * STAGE > STRIPS ? 2 * STAGE : STRIPS];
+    static_assert(2 * STAGE <= gemm_lds<T, WI, WJ, MI, MJ>, "two stages");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = wave / WJ, wj = wave % WJ;
 
     // Workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, so that the tiles sharing an
     // operand share an L2.
-    int id = blockIdx.x;
     const int total = g.tiles_i * g.tiles_j * g.splits, per = total >> 3, rest = total & 7, xcd = id & 7;
     id = xcd * per + min(xcd, rest) + (id >> 3);
     const int split = id / (g.tiles_i * g.tiles_j);
@@ -499,6 +500,26 @@ __global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
     }
 }
 
+template <class T, bool ARC, bool BRC, int WI, int WJ, int MI, int MJ, bool DIRECT>
+__global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_kernel(GemmArgs g)
+{
+    __shared__ __align__(128) char lds[gemm_lds<T, WI, WJ, MI, MJ>];
+    gemm_tile<T, ARC, BRC, WI, WJ, MI, MJ, DIRECT>(g, blockIdx.x, lds);
+}
+
+// Both products of the backward in one launch: first the one whose workgroups take longer (more steps of r each), then
+// the other's, which fill up the CUs as those run out.
+template <class T, int WI, int WJ, int MI, int MJ, bool DIRECT>
+__global__ void __launch_bounds__(WI * WJ * 64) dense_gemm_pair_kernel(GemmArgs dx, GemmArgs dw, int dx0, int dw0)
+{
+    __shared__ __align__(128) char lds[gemm_lds<T, WI, WJ, MI, MJ>];
+    // (one of dx0, dw0, the products' first workgroups, is 0)
+    if ((int)blockIdx.x >= dx0 && (dx0 || (int)blockIdx.x < dw0))
+        gemm_tile<T, true, false, WI, WJ, MI, MJ, DIRECT>(dx, blockIdx.x - dx0, lds);
+    else
+        gemm_tile<T, false, false, WI, WJ, MI, MJ, DIRECT>(dw, blockIdx.x - dw0, lds);
+}
+
 // The column sums' shares added up, by 256 threads: 16 columns, 16 lanes a column.
 template <class T>
 __device__ __forceinline__ void join_sums(const float *part, int parts, long long n, T *out, long long block)
@@ -522,18 +543,28 @@ __device__ __forceinline__ void join_sums(const float *part, int parts, long lon
     }
 }
 
-// Adds the shares of r in order and runs the epilogue; a thread takes eight columns of a row.  The workgroups behind
-// those, if any, add the column sums' shares.
+// Adds the shares of r in order and runs the epilogue, for one product or two; a thread takes eight columns of a row.
+// The workgroups behind those, if any, add the second (or only) one's column sums' shares.
+struct JoinArgs {
+    GemmArgs g[2];
+    unsigned blocks[2], sum_blocks;
+};
+
 template <class T>
-__global__ void __launch_bounds__(256) dense_gemm_join_kernel(GemmArgs g, unsigned blocks)
+__global__ void __launch_bounds__(256) dense_gemm_join_kernel(JoinArgs a)
 {
-    if (blockIdx.x >= blocks) {
-        join_sums<T>(g.colsum, g.splits * g.sharers, g.I, static_cast<T *>(g.colsum_out), blockIdx.x - blocks);
+    unsigned block = blockIdx.x;
+    const int which = block >= a.blocks[0];
+    if (which)
+        block -= a.blocks[0];
+    const GemmArgs &g = a.g[which];
+    if (which && block >= a.blocks[1]) {
+        join_sums<T>(g.colsum, g.splits * g.sharers, g.I, static_cast<T *>(g.colsum_out), block - a.blocks[1]);
         return;
     }
     const uint64_t seed = dn_seed(g.e.drop);
     const uint32_t units = (uint32_t)(g.pitch / 8);
-    const uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t u = (uint64_t)block * 256 + threadIdx.x;
     const uint64_t row = u / units;
     const uint32_t col = (uint32_t)(u - row * units) * 8;
     if (row >= (uint64_t)g.I)
@@ -654,6 +685,7 @@ struct Plan {
     long long pitch;
     size_t bytes;                // of the fp32 shares
     int sharers;                 // of the column sums
+    double cost;                 // the estimate
 };
 
 // The tiles a workgroup can make, rows x columns of C, the workgroups of a kind that fit a CU together (by LDS), and what
@@ -669,7 +701,8 @@ constexpr TileKind TILES[] = {{64, 64, 4, 330, 1350}, {128, 128, 2, 800, 4700}, 
 // a further kernel.
 constexpr double ARRIVE = 1400, START_END = 8000, JOIN = 14000, JOIN_BYTES = 2000;
 
-Plan plan(int type, long long I, long long J, long long R)
+// `only`: that kind of tile.
+Plan plan(int type, long long I, long long J, long long R, int only = -1)
 {
     Plan p = {};
     p.splits = 1;
@@ -679,8 +712,10 @@ Plan plan(int type, long long I, long long J, long long R)
     p.pitch = dn_ceil(J, 8) * 8;
     const int most = p.steps / 2 < 64 ? p.steps / 2 : 64;
     const bool fp32 = type == OPUS_DENSE_F32;
-    double best = 0;
+    double &best = p.cost;
     for (int k = 0; k < 3; ++k) {
+        if (only >= 0 && k != only)
+            continue;
         const TileKind &t = TILES[k];
         const long long tiles = dn_ceil(I, t.i) * dn_ceil(J, t.j);
         // no cut, and the cuts that give every CU 1, 2, ... workgroups, up to two turns
@@ -731,37 +766,61 @@ void launch_tiles(const Plan &p, const GemmArgs &g, hipStream_t s)
         hipLaunchKernelGGL((dense_gemm_kernel<T, ARC, BRC, 2, 2, 1, 1, DIRECT>), grid, dim3(256), 0, s, g);
 }
 
-// C = A B^T with an epilogue; `shares`: p.bytes of workspace.  sums_out [I]: the sums over r of A(i, r), or NULL; `sums`:
-// [p.splits * p.sharers][I] of workspace for them.
+// C = A B^T with an epilogue, planned as `p`.  shares: p.bytes of workspace.  sums_out [I]: the sums over r of A(i, r), or
+// NULL; sums: [p.splits * p.sharers][I] of workspace for them.
+struct Product {
+    GemmArgs g;
+    bool direct;
+    long long blocks;
+};
+
 template <class T, bool ARC, bool BRC>
-hipError_t gemm(int type, const void *a, const void *b, long long I, long long J, long long R, const Epilogue &e,
-                float *shares, float *sums, void *sums_out, hipStream_t s)
+Product product(const Plan &p, const void *a, const void *b, long long I, long long J, long long R, const Epilogue &e,
+                float *shares, float *sums, void *sums_out)
 {
-    const Plan p = plan(type, I, J, R);
-    if ((long long)p.tiles_i * p.tiles_j * p.splits * 256 > 0xFFFFFFFFll)
-        return hipErrorInvalidValue;
-    GemmArgs g = {a, b, I, J, R, p.tiles_i, p.tiles_j, p.splits, p.steps, p.steps_per_split,
-                  p.splits > 1 ? shares : nullptr, p.pitch, p.splits * p.sharers > 1 ? sums : nullptr, sums_out, p.sharers, e};
     const int piece = Elem<T>::PIECE;
     // (a tile's pieces are addressed in 32 bits from its corner)
     const auto near = [](bool rc, long long i, long long r) { return (rc ? 256 * r : 64 * i) * sizeof(T) < (1ll << 31); };
-    const bool direct = aligned16(a) && aligned16(b) && (ARC ? R : I) % piece == 0 && (BRC ? R : J) % piece == 0 &&
-                        near(ARC, I, R) && near(BRC, J, R);
-    if (direct)
-        launch_tiles<T, ARC, BRC, true>(p, g, s);
-    else
-        launch_tiles<T, ARC, BRC, false>(p, g, s);
-    const long long sum_blocks = sums_out && g.colsum ? dn_ceil(I, 16) : 0;
-    if (p.splits > 1) {
-        const long long blocks = dn_ceil(I * (p.pitch / 8), 256);
-        if ((blocks + sum_blocks) * 256 > 0xFFFFFFFFll)
-            return hipErrorInvalidValue;
-        hipLaunchKernelGGL(dense_gemm_join_kernel<T>, dim3((unsigned)(blocks + sum_blocks)), dim3(256), 0, s, g, (unsigned)blocks);
-    } else if (sum_blocks) {
-        hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)sum_blocks), dim3(256), 0, s, g.colsum, p.sharers, I,
-                           static_cast<T *>(sums_out));
+    return {{a, b, I, J, R, p.tiles_i, p.tiles_j, p.splits, p.steps, p.steps_per_split, p.splits > 1 ? shares : nullptr, p.pitch,
+             p.splits * p.sharers > 1 ? sums : nullptr, sums_out, p.sharers, e},
+            aligned16(a) && aligned16(b) && (ARC ? R : I) % piece == 0 && (BRC ? R : J) % piece == 0 && near(ARC, I, R) && near(BRC, J, R),
+            (long long)p.tiles_i * p.tiles_j * p.splits};
+}
+
+// What is left to do behind one product or two (NULL): shares to add, and the second one's column sums.
+template <class T>
+hipError_t join(const GemmArgs *one, const GemmArgs &two, hipStream_t s)
+{
+    JoinArgs a = {};
+    long long blocks[2] = {0, 0};
+    if (one && one->splits > 1) {
+        a.g[0] = *one;
+        blocks[0] = dn_ceil(one->I * (one->pitch / 8), 256);
     }
+    a.g[1] = two;
+    if (two.splits > 1)
+        blocks[1] = dn_ceil(two.I * (two.pitch / 8), 256);
+    const long long sums = two.colsum_out && two.colsum ? dn_ceil(two.I, 16) : 0, all = blocks[0] + blocks[1] + sums;
+    if (all * 256 > 0xFFFFFFFFll)
+        return hipErrorInvalidValue;
+    a.blocks[0] = (unsigned)blocks[0];
+    a.blocks[1] = (unsigned)blocks[1];
+    a.sum_blocks = (unsigned)sums;
+    if (all)
+        hipLaunchKernelGGL(dense_gemm_join_kernel<T>, dim3((unsigned)all), dim3(256), 0, s, a);
     return hipSuccess;
+}
+
+template <class T, bool ARC, bool BRC>
+hipError_t gemm(const Plan &p, const Product &q, hipStream_t s)
+{
+    if (q.blocks * (p.tile == 2 ? 512 : 256) > 0xFFFFFFFFll)
+        return hipErrorInvalidValue;
+    if (q.direct)
+        launch_tiles<T, ARC, BRC, true>(p, q.g, s);
+    else
+        launch_tiles<T, ARC, BRC, false>(p, q.g, s);
+    return join<T>(nullptr, q.g, s);
 }
 
 // runs of rows of dense_colsum_kernel
@@ -774,22 +833,70 @@ long long colsum_runs(long long M, long long N)
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// The backward's two products, as they are planned where both are wanted: side by side in one launch if their tiles
+// are of one of the kinds of four waves (then of the kind that is cheaper for both).
+struct PlanPair {
+    Plan dx, dw;
+    bool together;
+};
+
+PlanPair plan_pair(int type, long long M, long long N, long long K)
+{
+    PlanPair p = {plan(type, M, K, N), plan(type, N, K, M), false};
+    if (M > 0 && N > 0 && K > 0 && p.dx.tile < 2 && p.dw.tile < 2) {
+        if (p.dx.tile != p.dw.tile) {
+            const PlanPair a = {plan(type, M, K, N, 0), plan(type, N, K, M, 0), false};
+            const PlanPair b = {plan(type, M, K, N, 1), plan(type, N, K, M, 1), false};
+            p = a.dx.cost + a.dw.cost < b.dx.cost + b.dw.cost ? a : b;
+        }
+        p.together = true;
+    }
+    return p;
+}
+
+size_t sums_bytes(const Plan &p, long long N) { return (size_t)p.splits * p.sharers * N * sizeof(float); }
+
 template <class T>
 hipError_t backward(int type, const void *dz, const void *x, const void *w, long long M, long long N, long long K,
                     void *dx, void *dw, void *db, float *ws, hipStream_t s)
 {
+    const bool want_dx = dx && M && K, want_dw = dw && N && K;
+    const Epilogue ex = {nullptr, nullptr, dx, nullptr, OPUS_DENSE_ACT_NONE, {}}, ew = {nullptr, nullptr, dw, nullptr, OPUS_DENSE_ACT_NONE, {}};
+    if (want_dx && want_dw) {
+        const PlanPair p = plan_pair(type, M, N, K);
+        if (p.together) {
+            float *const shares = ws + align256(p.dx.bytes) / sizeof(float), *const sums = shares + align256(p.dw.bytes) / sizeof(float);
+            const Product qx = product<T, true, false>(p.dx, dz, w, M, K, N, ex, ws, nullptr, nullptr);
+            const Product qw = product<T, false, false>(p.dw, dz, x, N, K, M, ew, shares, sums, db);
+            const long long blocks = qx.blocks + qw.blocks;
+            if (blocks * 256 > 0xFFFFFFFFll)
+                return hipErrorInvalidValue;
+            const dim3 grid((unsigned)blocks);
+            const bool dw_first = p.dw.steps_per_split > p.dx.steps_per_split;
+            const int dx0 = dw_first ? (int)qw.blocks : 0, dw0 = dw_first ? 0 : (int)qx.blocks;
+            const bool direct = qx.direct && qw.direct;
+            if (p.dx.tile == 1 && direct)
+                hipLaunchKernelGGL((dense_gemm_pair_kernel<T, 2, 2, 2, 2, true>), grid, dim3(256), 0, s, qx.g, qw.g, dx0, dw0);
+            else if (p.dx.tile == 1)
+                hipLaunchKernelGGL((dense_gemm_pair_kernel<T, 2, 2, 2, 2, false>), grid, dim3(256), 0, s, qx.g, qw.g, dx0, dw0);
+            else if (direct)
+                hipLaunchKernelGGL((dense_gemm_pair_kernel<T, 2, 2, 1, 1, true>), grid, dim3(256), 0, s, qx.g, qw.g, dx0, dw0);
+            else
+                hipLaunchKernelGGL((dense_gemm_pair_kernel<T, 2, 2, 1, 1, false>), grid, dim3(256), 0, s, qx.g, qw.g, dx0, dw0);
+            return join<T>(&qx.g, qw.g, s);
+        }
+    }
     hipError_t e = hipSuccess;
-    if (dx && M && K) {
-        const Epilogue ep = {nullptr, nullptr, dx, nullptr, OPUS_DENSE_ACT_NONE, {}};
-        e = gemm<T, true, false>(type, dz, w, M, K, N, ep, ws, nullptr, nullptr, s);
+    if (want_dx) {
+        const Plan p = plan(type, M, K, N);
+        e = gemm<T, true, false>(p, product<T, true, false>(p, dz, w, M, K, N, ex, ws, nullptr, nullptr), s);
     }
     if (e != hipSuccess)
         return e;
-    const Plan p = plan(type, N, K, M);
-    float *sums = ws + align256(p.bytes) / sizeof(float);
-    if (dw && N && K) {
-        const Epilogue ep = {nullptr, nullptr, dw, nullptr, OPUS_DENSE_ACT_NONE, {}};
-        e = gemm<T, false, false>(type, dz, x, N, K, M, ep, ws, sums, db, s);
+    if (want_dw) {
+        const Plan p = plan(type, N, K, M);
+        float *const sums = ws + align256(p.bytes) / sizeof(float);
+        e = gemm<T, false, false>(p, product<T, false, false>(p, dz, x, N, K, M, ew, ws, sums, db), s);
     } else if (db && N) {
         const long long runs = colsum_runs(M, N), per = dn_ceil(M > 0 ? M : 1, runs);
         hipLaunchKernelGGL(dense_colsum_kernel<T>, dim3((unsigned)dn_ceil(N, 32), (unsigned)runs), dim3(256), 0, s,
@@ -797,7 +904,7 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
         hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 16)), dim3(256), 0, s, ws,
                            (int)runs, N, static_cast<T *>(db));
     }
-    return hipSuccess;
+    return e;
 }
 
 }  // namespace
@@ -811,8 +918,10 @@ template <class T>
 static hipError_t forward(int type, const void *x, const void *w, long long M, long long N, long long K, const Epilogue &e,
                           float *workspace, hipStream_t s)
 {
-    if (M > FEW_ROWS)
-        return gemm<T, true, true>(type, x, w, M, N, K, e, workspace, nullptr, nullptr, s);
+    if (M > FEW_ROWS) {
+        const Plan p = plan(type, M, N, K);
+        return gemm<T, true, true>(p, product<T, true, true>(p, x, w, M, N, K, e, workspace, nullptr, nullptr), s);
+    }
     if (dn_ceil(N, 16) * 256 > 0xFFFFFFFFll)
         return hipErrorInvalidValue;
     const dim3 grid((unsigned)dn_ceil(N, 16));
@@ -843,12 +952,15 @@ size_t dn_linear_backward_workspace(int type, long long M, long long N, long lon
 {
     if (N <= 0)
         return 0;
-    const size_t x = M > 0 && K > 0 ? plan(type, M, K, N).bytes : 0;
-    const Plan p = plan(type, N, K, M);
-    const size_t w = align256(p.bytes) + (size_t)p.splits * p.sharers * N * sizeof(float);
-    const size_t alone = (size_t)colsum_runs(M, N) * N * sizeof(float);
-    const size_t most = x > w ? x : w;
-    return most > alone ? most : alone;
+    const Plan px = plan(type, M, K, N), pw = plan(type, N, K, M);
+    const PlanPair both = plan_pair(type, M, N, K);
+    size_t most = px.bytes;
+    const auto at_least = [&](size_t n) { most = most > n ? most : n; };
+    at_least(align256(pw.bytes) + sums_bytes(pw, N));
+    at_least((size_t)colsum_runs(M, N) * N * sizeof(float));
+    if (both.together)
+        at_least(align256(both.dx.bytes) + align256(both.dw.bytes) + sums_bytes(both.dw, N));
+    return most;
 }
 
 hipError_t dn_launch_linear_backward(int type, const void *dz, const void *x, const void *w, long long M,

@@ -12,7 +12,8 @@ Common to the three: tensors are fp32, bf16 or fp16, all of one type, on one GPU
 statistics and the epilogue are in fp32 and every result is rounded once.  A tensor that is not contiguous is copied
 first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep no
 state and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
-inputs give the same bits.  Gradients are first-order only.
+call on the same inputs gives the same bits (asking for other gradients along with one may round that one otherwise).
+Gradients are first-order only.
 
 ``D`` is dropout with a counter-based generator: whether element (row, column) is kept is computed from
 ``(seed, offset, row, column)`` - row counting the tensor's last-dimension rows - by Philox 4x32-10, in the forward
@@ -58,13 +59,13 @@ def _threshold(what, p, seed, offset, device):
     """p -> threshold of 65536 (0: no dropout); checks the generator's arguments."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{what}: dropout probability has to be between 0 and 1, got {p}")
-    threshold = round(p * 65536)
+    threshold = round(float(p) * 65536)
     if threshold == 0:
         return 0
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise RuntimeError(f"{what}: a seed tensor has to hold one int64 on {device}")
-    elif not isinstance(seed, int) or isinstance(seed, bool):
+    elif not hasattr(seed, "__index__") or isinstance(seed, bool):
         raise RuntimeError(f"{what}: dropout needs a seed, an int or a one-element int64 tensor")
     if not 0 <= offset < 2 ** 32:
         raise ValueError(f"{what}: offset has to be in [0, 2**32), got {offset}")
@@ -75,8 +76,8 @@ def _drop_struct(threshold, seed, offset):
     if threshold == 0:
         return None
     if isinstance(seed, torch.Tensor):
-        return _lib.DenseDropout(threshold, offset, 0, seed.data_ptr())
-    return _lib.DenseDropout(threshold, offset, seed & (2 ** 64 - 1), None)
+        return _lib.DenseDropout(threshold, int(offset), 0, seed.data_ptr())
+    return _lib.DenseDropout(threshold, int(offset), int(seed) & (2 ** 64 - 1), None)
 
 
 def _seed_tensor(threshold, seed):
@@ -331,6 +332,11 @@ def residual_norm(x, block, weight=None, bias=None, kind="layer", eps=1e-5, post
     code = _lib.DENSE_NORMS.get(kind)
     if code is None:
         raise ValueError(f"residual_norm: kind has to be one of {sorted(_lib.DENSE_NORMS)}, got {kind!r}")
+    if isinstance(residual_scale, torch.Tensor) or isinstance(eps, torch.Tensor):
+        raise RuntimeError("residual_norm: residual_scale and eps are numbers, not tensors (no gradient would reach them)")
+    eps, residual_scale = float(eps), float(residual_scale)
+    if not eps >= 0.0:
+        raise ValueError(f"residual_norm: eps has to be no less than 0, got {eps}")
     gate_rows = 0 if gate is None else _gate_rows(x, gate)
     threshold = _threshold("residual_norm", dropout_p, seed, offset, x.device) if dropout_p != 0.0 else 0
     if _wants_grad(tensors):

@@ -140,6 +140,10 @@ def test_dropout_threshold_and_seed_checks():
     assert _threshold("d", 0.1, -1, 0, cpu) == 6554
     assert _threshold("d", 1.0, 7, 2 ** 32 - 1, cpu) == 65536
     assert _threshold("d", 2.0 ** -18, None, 0, cpu) == 0
+    assert _threshold("d", np.float32(0.5), np.int64(3), np.int32(2), cpu) == 32768
+    from opus_amd.opus_dense import _drop_struct
+    drop = _drop_struct(32768, np.int64(-3), np.int32(2))
+    assert (drop.seed, drop.offset) == (2 ** 64 - 3, 2)
     assert _threshold("d", 0.5, torch.zeros(1, dtype=torch.int64), 0, cpu) == 32768
     for p in (-0.1, 1.1, float("nan")):
         with pytest.raises(ValueError):

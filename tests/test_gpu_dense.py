@@ -650,7 +650,8 @@ def test_refusals(od):
            lambda: od.linear(x, w, dropout_p=1.5, seed=1), lambda: od.linear(x, w, dropout_p=0.5, seed=1, offset=-1),
            lambda: od.residual_norm(x, x[:2]), lambda: od.residual_norm(x, x, w), lambda: od.residual_norm(x, x, kind="batch"),
            lambda: od.residual_norm(x, x, post_bias=x[0]), lambda: od.residual_norm(x, x, gate=x[:3]),
-           lambda: od.residual_norm(x, x.half()), lambda: od.residual_norm(x[:, :0], x[:, :0]),
+           lambda: od.residual_norm(x, x, residual_scale=torch.ones((), device="cuda")), lambda: od.residual_norm(x, x, eps=-1.0),
+           lambda: od.residual_norm(x, x, eps=float("nan")), lambda: od.residual_norm(x, x.half()), lambda: od.residual_norm(x[:, :0], x[:, :0]),
            lambda: od.residual_norm(torch.zeros(1, 16385, device="cuda"), torch.zeros(1, 16385, device="cuda")),
            lambda: od.dropout(x, 0.5, None), lambda: od.dropout(x, -0.5, 1), lambda: od.dropout(x, 0.5, 1, residual=x[0]),
            lambda: od.dropout(x.int(), 0.5, 1)]
@@ -662,6 +663,93 @@ def test_refusals(od):
 
 def test_no_second_derivatives(od):
     x = torch.randn(4, 16, device="cuda", requires_grad=True)
-    g, = torch.autograd.grad(od.dropout(x, 0.5, 1).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    w = torch.randn(16, 16, device="cuda")
+    for f in (lambda: od.dropout(x, 0.5, 1), lambda: od.linear(x, w, activation="silu"), lambda: od.residual_norm(x, x)):
+        g, = torch.autograd.grad((f() ** 2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+def test_one_dimension_and_no_gradient_modes(od):
+    rng = np.random.default_rng(7)
+    x, w = make(rng, torch.float32, 40).requires_grad_(True), make(rng, torch.float32, 24, 40)
+    y = od.linear(x, w)
+    assert y.shape == (24,) and y.requires_grad
+    want, bound = linear_bounds(f64(x)[None], f64(w), None, None, None, "none", 1.0, torch.float32)
+    check(y[None], want, bound, "one dimension")
+    with torch.no_grad():
+        assert not od.linear(x, w).requires_grad and not od.dropout(x, 0.5, 1).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(od.linear(x, w), y.detach())
+    n = od.residual_norm(x, x, gate=x)
+    assert n.shape == (40,)
+    n.sum().backward()
+    assert x.grad.shape == (40,)
+    assert od.dropout(torch.zeros(3, 0, device="cuda"), 0.5, 1).shape == (3, 0)
+
+
+def test_backward_twice_and_inputs_changed_in_between(od):
+    rng = np.random.default_rng(8)
+    x, w = make(rng, torch.float32, 30, 40).requires_grad_(True), make(rng, torch.float32, 24, 40).requires_grad_(True)
+    y = od.linear(x, w, activation="gelu", dropout_p=0.2, seed=3)
+    a = torch.autograd.grad(y.sum(), [x, w], retain_graph=True)
+    b = torch.autograd.grad(y.sum(), [x, w], retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+
+
+def test_threads_at_once(od):
+    """Calls from several host threads, each on a stream of its own."""
+    import threading
+    t = layer_tensors()
+    want = layer(od, t, 4)
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = layer(od, t, 4)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_offsets_beyond_32_bits(od):
+    """Matrices of more than 2^32 bytes and 2^31 elements: the last rows are what the same rows give by themselves."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GiB of device memory")
+    gen = torch.Generator("cuda").manual_seed(2)
+    n = lambda *s: torch.randn(s, generator=gen, device="cuda", dtype=torch.bfloat16)       # noqa: E731
+    M, K, N, tail = 70000, 64, 40000, 300                                        # 2.8e9 outputs
+    x, w, b = n(M, K), n(N, K), n(N)
+    y = od.linear(x, w, b, activation="relu")
+    part = od.linear(x[-tail:], w, b, activation="relu")
+    err = (y[-tail:].float() - part.float()).abs()
+    assert (err <= 2 * U[torch.bfloat16] * part.float().abs() + (K + 2) * STEP * 64).all()   # (another plan's order of sums)
+    del y, part, err
+    dy = n(M, N)
+    xr = x.requires_grad_(True)
+    dx, = torch.autograd.grad(od.linear(xr, w), xr, dy)
+    ref = dy[-tail:].float() @ w.float()
+    # fp32 sums of N terms of about 1 on both sides, then one rounding
+    assert ((dx[-tail:].float() - ref).abs() <= U[torch.bfloat16] * ref.abs() * 1.01 + 2 * (N + 2) * STEP * N ** 0.5).all()
+    del dy, dx, ref
+    rows, width = 2 ** 19 + 3, 8200                                              # 4.3e9 elements
+    x = torch.empty(rows, width, device="cuda", dtype=torch.bfloat16)
+    block = torch.empty_like(x)
+    for t in (x, block):
+        t.normal_(generator=gen)
+    y = od.residual_norm(x, block, dropout_p=0.0)
+    assert torch.equal(y[-70:], od.residual_norm(x[-70:], block[-70:]))
+    d = od.dropout(x, 0.5, 9)
+    k = torch.from_numpy(do.keep(5, width, 0.5, 9, first_row=rows - 5)).cuda()
+    assert torch.equal(d[-5:].double(), x[-5:].double() * k)

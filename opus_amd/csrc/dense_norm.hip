@@ -237,12 +237,16 @@ __device__ __forceinline__ void flush(O *out, Row<CH, VEC> &acc, float *cols, in
 }
 
 // POST: with a post-norm.  BIAS: a bias' gradient may be wanted.  A workgroup works on rows_per_group consecutive rows of one gate row where chunks > 1,
-// otherwise on rows_per_group whole gate rows.  The next row's values are on their way while a row is worked on.
+// otherwise on rows_per_group whole gate rows.  AHEAD: the next row's
+// values are on their way while a row is worked on.
 template <class T, int TPR, int VEC, int CH, bool WHOLE, bool POST, bool BIAS>
 __global__ void __launch_bounds__(group_threads(TPR)) dense_norm_backward_kernel(NormArgs a)
 {
     constexpr int ROWS = group_threads(TPR) / TPR;
-    constexpr bool KEEP = sizeof(T) * VEC * CH <= 16, AHEAD = CH == 1 || (TPR < 1024 && sizeof(T) == 2);
+    constexpr bool KEEP = sizeof(T) * VEC * CH <= 16;
+    // (not where the next row's registers would spill: 8192 x 8192 bf16 with a post-norm 337 us ahead, 376 not, but with
+    // biases as well 454 and 421; 8 elements a thread of 1024 threads instead of 16 of 512: 397 and up)
+    constexpr bool AHEAD = CH == 1 || (TPR < 1024 && sizeof(T) == 2 && !(POST && BIAS));
     __shared__ float lds[64];
     __shared__ __align__(16) float cols[ROWS > 1 ? ROWS * TPR * VEC : 4];
     int phase = 0;

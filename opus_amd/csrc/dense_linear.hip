@@ -19,6 +19,13 @@
 // one row: 16-byte accesses to bias, residual, z and y, and one generator call of the dropout for the eight.  Few
 // tiles and a long r: r is cut up over workgroups, each stores its fp32 share, and a second kernel adds the shares in
 // order and runs the epilogue.  No atomics: the result does not depend on the order of the workgroups.
+//
+// Measured on one MI355X (the library's plain products in brackets): 8192 x 4096 x 4096 bf16 forward 225 us = 1220 TFLOP/s
+// (196), dx 221 (217), dW 221 (247); 4096^3 fp32 965 us = 142 TFLOP/s; 4800 x 256 -> 18432 bf16 forward 97 (96),
+// both gradients 132 (214); 4800 x 8192 -> 256 fp32 forward 189 (228), both gradients 335 (342).  The wide tile's matrix
+// cores are busy 59 % of its cycles, LDS 24 %: without the transfers, or without the reads of LDS, it would be 15 % faster
+// each, so both have to run beside the matrix instructions, which are interleaved with them.  With few steps of r (256)
+// start and epilogue weigh as much as the product.
 #include "dense_common.h"
 
 namespace {
@@ -909,16 +916,29 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
 
 }  // namespace
 
+// Few rows take their own kernel rather than tiles (1 row, 1024 -> 4096 bf16: 4.6 us and 8.4; 16 rows, 4096 -> 4096: 11.6
+// and 14.3; 1 row, 8192 -> 8192 fp32: 52 and 85), but for two shapes: few columns over long rows of W, which leave most of
+// the chip idle (1 row, 8192 -> 256 fp32: 19.7 and 16.1), and many 16-bit rows over a large W, where reading x again for
+// every 16 columns shows (16 rows, 8192 -> 8192 bf16: 39 and 31).
+static bool few_rows(int type, long long M, long long N, long long K)
+{
+    if (M > FEW_ROWS)
+        return false;
+    if (N <= 1024 && K * (long long)dn_type_bytes(type) >= 32768)
+        return false;
+    return type == OPUS_DENSE_F32 || M <= 8 || N * K < (1ll << 25);
+}
+
 size_t dn_linear_forward_workspace(int type, long long M, long long N, long long K)
 {
-    return M > FEW_ROWS && N > 0 ? plan(type, M, N, K).bytes : 0;
+    return M > 0 && N > 0 && !few_rows(type, M, N, K) ? plan(type, M, N, K).bytes : 0;
 }
 
 template <class T>
 static hipError_t forward(int type, const void *x, const void *w, long long M, long long N, long long K, const Epilogue &e,
                           float *workspace, hipStream_t s)
 {
-    if (M > FEW_ROWS) {
+    if (!few_rows(type, M, N, K)) {
         const Plan p = plan(type, M, N, K);
         return gemm<T, true, true>(p, product<T, true, true>(p, x, w, M, N, K, e, workspace, nullptr, nullptr), s);
     }

@@ -10,6 +10,11 @@
 // statistics.  Sums over rows (dweight, dbias, dpost_*, dgate) stay in each thread's registers while its workgroup
 // walks a run of rows, are stored once a workgroup as fp32 rows, and a second small kernel adds those up: no atomics,
 // the same order every time.  All sums are in fp32.
+//
+// Measured on one MI355X: 38400 x 256 fp32 LayerNorm with dropout 30 us forward (157 MB, 5.2 TB/s), 40 backward (236 MB,
+// 5.9 TB/s) and 6 for the sums over rows; 8192 x 8192 bf16 RMS with post-norm and a gate a sample 117 forward (537 MB,
+// 4.6 TB/s), 226 backward (805 MB, 3.6 TB/s: a row of 8192 with five gradients in flight fills a CU's registers, so only
+// one is worked on and one under way) and 11.
 #include "dense_common.h"
 
 namespace {

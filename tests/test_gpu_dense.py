@@ -135,6 +135,8 @@ def test_linear_few_rows(od, dtype):
     run_linear(od, 120, TYPES[dtype], 1, 8200, 4096, name="silu", train=False)
     run_linear(od, 121, TYPES[dtype], 3, 4099, 57, train=False)
     run_linear(od, 122, TYPES[dtype], 16, 2048, 9001, train=False)
+    run_linear(od, 123, TYPES[dtype], 2, 8192, 40, train=False)                # few columns over long rows: tiles in fp32
+    run_linear(od, 124, TYPES[dtype], 9, 4104, 8200, train=False)              # nine rows over a large W: tiles in 16 bits
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))

@@ -252,10 +252,12 @@ __device__ __forceinline__ float add_up(f32x4 v, float s) { return s + ((v[0] + 
 
 constexpr int STRIP = 72;       // floats a row of a wave's strip in LDS: rows four apart then start 32 banks apart
 
-// WI x WJ waves, each MI x MJ blocks of 32 x 32.  DIRECT: bases and rows are 16-byte aligned.
+// LDS of a workgroup: two stages of both operands' tiles, and in their place the epilogue's strips
 template <class T, int WI, int WJ, int MI, int MJ>
-constexpr int gemm_lds = (2 * (WI * MI + WJ * MJ) * 32 * 128 > WI * WJ * 32 * STRIP * 4) ? 2 * (WI * MI + WJ * MJ) * 32 * 128 : WI * WJ * 32 * STRIP * 4;
+constexpr int gemm_lds = (2 * (WI * MI + WJ * MJ) * 32 * 128 > WI * WJ * 32 * STRIP * 4) ? 2 * (WI * MI + WJ * MJ) * 32 * 128
+                                                                                        : WI * WJ * 32 * STRIP * 4;
 
+// Workgroup `id` of a product: WI x WJ waves, each MI x MJ blocks of 32 x 32.  DIRECT: bases and rows are 16-byte aligned.
 template <class T, bool ARC, bool BRC, int WI, int WJ, int MI, int MJ, bool DIRECT>
 __device__ __forceinline__ void gemm_tile(const GemmArgs &g, int id, char *lds)
 {

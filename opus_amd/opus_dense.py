@@ -86,6 +86,12 @@ def _seed_tensor(threshold, seed):
     return seed if threshold and isinstance(seed, torch.Tensor) else None
 
 
+def _drop_again(drop, seed):
+    """The forward's dropout for the backward: with the seed tensor autograd hands back, which need not lie where the
+    forward's did (saved-tensor hooks may have moved it)."""
+    return drop if seed is None else _lib.DenseDropout(drop.threshold, drop.offset, 0, seed.data_ptr())
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -172,8 +178,9 @@ class _Linear(torch.autograd.Function):
 
     @_first_order
     def backward(ctx, dy):
-        x, weight, z, _ = ctx.saved_tensors
+        x, weight, z, seed = ctx.saved_tensors
         activation, drop = ctx.settings
+        drop = _drop_again(drop, seed)
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
@@ -261,6 +268,7 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 8
         saved = ctx.saved_tensors
         kind, gate_rows, eps, scale, drop = ctx.settings
+        drop = _drop_again(drop, saved[8])
         tensors, stats = [_contiguous(t) for t in saved[:7]], saved[7]
         grads = [torch.empty_like(t) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
         x = tensors[0]
@@ -370,9 +378,10 @@ class _Dropout(torch.autograd.Function):
 
     @_first_order
     def backward(ctx, dy):
-        ctx.saved_tensors                       # (a seed tensor that was changed since is an error)
+        saved = ctx.saved_tensors               # (a seed tensor that was changed since is an error)
+        drop = _drop_again(ctx.drop, saved[0]) if saved else ctx.drop
         need_x, need_r = ctx.needs_input_grad[:2]
-        return _dropout(dy, None, ctx.drop) if need_x else None, dy if need_r else None, None, None, None
+        return _dropout(dy, None, drop) if need_x else None, dy if need_r else None, None, None, None
 
 
 def dropout(x, p, seed, offset=0, residual=None):

@@ -6,6 +6,7 @@ for what a matrix instruction may drop inside) times the sum of the terms' magni
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oracle import dense_oracle as do
 
@@ -701,6 +702,33 @@ def test_backward_twice_and_inputs_changed_in_between(od):
         w.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y.sum(), x)
+
+
+def test_saved_tensors_that_move_and_checkpointing(od):
+    """Saved-tensor hooks hand the backward other tensors (the seed's among them); activation checkpointing runs the
+    forward again.  Both give the plain run's gradients, bit for bit."""
+    t = layer_tensors()
+    leaves = [v.requires_grad_(True) for v in t.values()]
+    grad = torch.randn_like(t["query"])
+
+    def grads(run):
+        y = run()
+        torch.full((64,), -1, device="cuda")                     # (what a freed seed's place may hold next)
+        return torch.autograd.grad(y, leaves, grad)
+
+    want = grads(lambda: od.dropout(layer(od, t, 8), 0.3, 8, 9))
+
+    def moved():
+        with torch.autograd.graph.save_on_cpu():
+            return od.dropout(layer(od, t, torch.tensor([8], device="cuda")), 0.3, torch.tensor([8], device="cuda"), 9)
+
+    def again():
+        seed = torch.tensor([8], device="cuda")
+        return torch.utils.checkpoint.checkpoint(lambda: od.dropout(layer(od, t, seed), 0.3, seed, 9), use_reentrant=False)
+
+    for run in (moved, again):
+        for a, b in zip(grads(run), want):
+            assert torch.equal(a, b)
 
 
 def test_threads_at_once(od):

@@ -176,7 +176,7 @@ __device__ __forceinline__ float dn_gelu_slope(float z)
 {
     return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
 }
-// s = (1 + tanh u) / 2;  s + 2 z s (1 - s) u'
+// s = (1 + tanh u) / 2;  s + 2 z s (1 - s) u'.
 __device__ __forceinline__ float dn_gelu_tanh_slope(float z)
 {
     const float z2 = z * z, s = 1.f / (1.f + expf(-1.59576912f * (z + 0.044715f * z * z2)));
@@ -188,15 +188,33 @@ __device__ __forceinline__ float dn_silu_slope(float z)
     return s * (1.f + z * (1.f - s));
 }
 
-// v[j] = act(v[j]); the choice is uniform and outside the loops
-template <int N> __device__ __forceinline__ void dn_act(dn_floats<N> &v, int act)
+// z / (1 + exp(-a)) with the hardware's exponential and reciprocal, for results that are rounded to 16 bits: its error is
+// within 2^-21 (1 + |a|) of the value against a half step of 2^-11 (fp16) or 2^-8 (bf16), and 0 instead of the 1e-36 that is
+// left below a = -87.  8192 x 4096 x 4096 bf16 with silu: 239 -> 223 us, with gelu_tanh 240 -> 226 us (228 without either).
+__device__ __forceinline__ float dn_gated_fast(float z, float a)
+{
+    return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * a));
+}
+
+// v[j] = act(v[j]), rounded to T next; the choice is uniform and outside the loops
+template <int N, class T> __device__ __forceinline__ void dn_act(dn_floats<N> &v, int act)
 {
 #define DN_EACH(expr) _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = expr
     switch (act) {
     case OPUS_DENSE_ACT_RELU: DN_EACH(dn_relu(v[j])); break;
     case OPUS_DENSE_ACT_GELU: DN_EACH(dn_gelu(v[j])); break;
-    case OPUS_DENSE_ACT_GELU_TANH: DN_EACH(dn_gelu_tanh(v[j])); break;
-    case OPUS_DENSE_ACT_SILU: DN_EACH(dn_silu(v[j])); break;
+    case OPUS_DENSE_ACT_GELU_TANH:
+        if constexpr (sizeof(T) == 4)
+            DN_EACH(dn_gelu_tanh(v[j]));
+        else
+            DN_EACH(dn_gated_fast(v[j], 1.59576912f * (v[j] + 0.044715f * v[j] * v[j] * v[j])));
+        break;
+    case OPUS_DENSE_ACT_SILU:
+        if constexpr (sizeof(T) == 4)
+            DN_EACH(dn_silu(v[j]));
+        else
+            DN_EACH(dn_gated_fast(v[j], v[j]));
+        break;
     default: break;
     }
 }

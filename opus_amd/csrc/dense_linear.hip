@@ -65,7 +65,7 @@ __device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, const 
                     z[j] = 6e-8f;
         dn_store_n<8>(static_cast<T *>(e.z) + at, z, n);
     }
-    dn_act<8>(v, e.act);
+    dn_act<8, T>(v, e.act);
     if (e.drop.threshold)
         dn_drop<8>(v, row, col, seed, e.drop);
     if (e.residual)

@@ -176,9 +176,10 @@ __device__ __forceinline__ float dn_gelu_slope(float z)
 {
     return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
 }
-// s = (1 + tanh u) / 2;  s + 2 z s (1 - s) u'.
+// s = (1 + tanh u) / 2;  s + 2 z s (1 - s) u'.  Beyond |z| = 16 s is 0 or 1, and z^2 may not become inf beside that zero.
 __device__ __forceinline__ float dn_gelu_tanh_slope(float z)
 {
+    z = z > 16.f ? 16.f : z < -16.f ? -16.f : z;                 // NaN stays
     const float z2 = z * z, s = 1.f / (1.f + expf(-1.59576912f * (z + 0.044715f * z * z2)));
     return s + 2.f * z * s * (1.f - s) * 0.79788456f * (1.f + 0.134145f * z2);
 }

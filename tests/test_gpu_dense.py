@@ -128,6 +128,33 @@ def test_linear_activations_with_dropout(od, dtype, name):
     run_linear(od, 51, TYPES[dtype], 3, 40, 264, name=name, p=0.0, train=False)
 
 
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES)
+def test_activation_and_slope_at_every_magnitude(od, dtype, name):
+    """z = x 1 is exact, so only the activation and the rounding of its result are off: every finite 16-bit number (every
+    65521st fp32 one).  a, the exponent's argument, carries a few roundings: 2^-21 |a| of the value; beyond |a| = 100 the
+    exponential is 0 or its term all that counts, and below -87 the value left, under 128 x 2^-126, may become 0.  erf's
+    error is absolute: 2^-21 |z| until it is 1 (|z| < 8).  The oracle's 1 + tanh in 64 bits is itself off by up to 2^-52
+    (tanh by an ulp below 1, and the sum's rounding) and so its value by |z| / 2 times that, until both are 0 or 2: at
+    |z| >= 8 what it loses is under |z| exp(-49).  The slopes' as in linear_bounds."""
+    if dtype == torch.float32:
+        x = torch.arange(-2 ** 31, 2 ** 31, 65521).to(torch.int32).view(dtype)
+    else:
+        x = torch.arange(-2 ** 15, 2 ** 15).to(torch.int16).view(dtype)
+    x = x[torch.isfinite(x)].reshape(-1, 1).cuda().requires_grad_()
+    z = f64(x)
+    with np.errstate(over="ignore"):
+        value, slope = do.act(z, name)
+    y = od.linear(x, torch.ones(1, 1, dtype=dtype, device="cuda"), activation=name)
+    y.backward(torch.ones_like(y))
+    a = {"gelu": 0, "silu": z, "gelu_tanh": 1.6 * (z + 0.044715 * z ** 3)}[name]
+    off = 2.0 ** -21 * (np.abs(value) * (1 + np.minimum(np.abs(a), 100)) + (name == "gelu") * np.minimum(np.abs(z), 8))
+    off += 2.0 ** -53 * (name == "gelu_tanh") * np.minimum(np.abs(z), 8)
+    check(y, value, off * (1 + U[dtype]) + rounded(value, dtype) + 2.0 ** -119, f"{name} value")
+    off = 32 * STEP * (1 + np.minimum(np.abs(z), 128))
+    check(x.grad, slope, off * (1 + U[dtype]) + 2 * rounded(slope, dtype), f"{name} slope")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
 def test_linear_few_rows(od, dtype):
     """Up to 16 rows of x go through a kernel of their own: both its widths, whole and odd lengths, every row count."""

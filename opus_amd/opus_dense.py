@@ -67,6 +67,8 @@ def _threshold(what, p, seed, offset, device):
             raise RuntimeError(f"{what}: a seed tensor has to hold one int64 on {device}")
     elif not hasattr(seed, "__index__") or isinstance(seed, bool):
         raise RuntimeError(f"{what}: dropout needs a seed, an int or a one-element int64 tensor")
+    if not hasattr(offset, "__index__") or isinstance(offset, (bool, torch.Tensor)):
+        raise RuntimeError(f"{what}: offset has to be an int, got {offset!r}")
     if not 0 <= offset < 2 ** 32:
         raise ValueError(f"{what}: offset has to be in [0, 2**32), got {offset}")
     return threshold

@@ -156,6 +156,14 @@ def test_dropout_threshold_and_seed_checks():
             _threshold("d", 0.5, 7, offset, cpu)
 
 
+def test_dropout_offset_is_an_int():
+    """1.2 and 1.7 would both have been offset 1: the same mask twice."""
+    from opus_amd.opus_dense import _threshold
+    for offset in (1.5, 1.0, True, None, torch.zeros((), dtype=torch.int64)):
+        with pytest.raises(RuntimeError):
+            _threshold("d", 0.5, 7, offset, torch.device("cpu"))
+
+
 def test_oracle_generator_against_published_vectors():
     """Known answers of philox4x32-10 (Random123's kat_vectors)."""
     ones = 0xFFFFFFFF

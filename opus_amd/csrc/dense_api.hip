@@ -65,7 +65,9 @@ int check_norm(const opus_dense_norm_t *in, DnDrop &drop)
         return OPUS_DENSE_EINVAL_TYPE;
     if (in->kind != OPUS_DENSE_NORM_LAYER && in->kind != OPUS_DENSE_NORM_RMS)
         return OPUS_DENSE_EINVAL_FLAGS;
-    if (in->rows < 0 || in->width < 1 || (in->gate && in->rows > 0 && (in->gate_rows < 1 || in->rows % in->gate_rows)))
+    // (a gate without rows goes with no rows at all)
+    if (in->rows < 0 || in->width < 1 || (in->gate && in->gate_rows < (in->rows > 0)) ||
+        (in->gate && in->rows > 0 && in->rows % in->gate_rows))
         return OPUS_DENSE_EINVAL_DIMS;
     if (in->width > OPUS_DENSE_MAX_WIDTH || in->rows > LLONG_MAX / 8 / in->width)
         return OPUS_DENSE_ETOOLARGE;

@@ -553,7 +553,7 @@ NormArgs common_args(const opus_dense_norm_t &in, const DnDrop &drop)
     a.x = in.x; a.block = in.block; a.weight = in.weight; a.bias = in.bias;
     a.post_weight = in.post_weight; a.post_bias = in.post_weight ? in.post_bias : nullptr; a.gate = in.gate;
     a.rows = in.rows;
-    a.gate_rows = in.gate ? in.gate_rows : 1;
+    a.gate_rows = in.gate && in.gate_rows > 0 ? in.gate_rows : 1;
     a.rows_per_gate = in.rows / a.gate_rows;
     a.width = (int)in.width;
     a.rms = in.kind == OPUS_DENSE_NORM_RMS;
@@ -624,7 +624,7 @@ hipError_t dn_launch_norm_backward(const opus_dense_norm_t &in, const DnDrop &dr
     add(a.part_b, out.dbias, 1, p.workgroups);
     add(a.part_pw, out.dpost_weight, 1, p.workgroups);
     add(a.part_pb, out.dpost_bias, 1, p.workgroups);
-    if (a.part_gate || in.rows == 0)
+    if (a.part_gate || (in.rows == 0 && in.gate_rows > 0))
         add(a.part_gate, out.dgate, p.groups_rows, in.rows ? p.chunks : 0);
     r.width = (int)in.width;
     long long groups = 1;

@@ -109,6 +109,21 @@ def test_norm_and_dropout_arguments(lib):
     assert drop(0, NULL, NULL, 0, 8, None, NULL, None) == 0 and drop(0, NULL, NULL, 8, 0, None, NULL, None) == 0
 
 
+def test_norm_gate_without_rows(lib):
+    """No rows and a gate of none: nothing to do, and nothing divided by the gate's rows; fewer than none is refused."""
+    from opus_amd import _lib
+
+    def struct(rows, gate_rows):
+        return _lib.DenseNorm(0, 0, rows, 8, gate_rows, 1e-5, 1.0, SOME.value, SOME.value, None, None, None, None, 4096, None)
+
+    def backward(rows, gate_rows):
+        grads = _lib.DenseNormGrads(*(None,) * 6 + (4096,))
+        return lib.opus_dense_norm_backward(struct(rows, gate_rows), SOME, NULL, SOME, grads, NULL, 0, None)
+
+    assert lib.opus_dense_norm_forward(struct(0, 0), SOME, NULL, NULL, None) == 0 and backward(0, 0) == 0
+    assert lib.opus_dense_norm_forward(struct(0, -1), SOME, NULL, NULL, None) == -2 and backward(0, -1) == -2
+
+
 def test_host_side_refuses_cpu_tensors_and_other_types():
     from opus_amd import opus_dense as od
     x, w = torch.zeros(2, 8), torch.zeros(4, 8)

@@ -81,7 +81,7 @@ int opus_dense_linear_forward(int type, const void *x, const void *weight, const
  * Its gradients: dz = D(dy) act'(z); dx [M, K] = dz W; dweight [N, K] = dz^T x; dbias [N] = sum over rows of dz.
  * Each of dx, dweight, dbias may be NULL (not computed).  z is needed with an activation.  dz is held in the
  * element type: `dz_buffer` [M, N] receives it where there is an activation or dropout (required then, where
- * anything is computed; without either, dz is dy itself).  d residual is dy.
+ * anything is computed; without either, dz is dy itself); dbias is summed before that rounding.  d residual is dy.
  */
 size_t opus_dense_linear_backward_workspace_bytes(int type, long long M, long long N, long long K);
 int opus_dense_linear_backward(int type, const void *dy, const void *x, const void *weight, const void *z,

@@ -162,13 +162,7 @@ int opus_dense_linear_backward(int type, const void *dy, const void *x, const vo
     rc = check_workspace(workspace, workspace_bytes, dn_linear_backward_workspace(type, M, N, K));
     if (rc != OPUS_DENSE_OK)
         return rc;
-    if (prepare) {
-        rc = status(dn_launch_elementwise(type, dy, nullptr, activation != OPUS_DENSE_ACT_NONE ? z : nullptr, activation,
-                                          M, N, drop, dz_buffer, (hipStream_t)stream));
-        if (rc != OPUS_DENSE_OK)
-            return rc;
-    }
-    return status(dn_launch_linear_backward(type, prepare ? dz_buffer : dy, x, weight, M, N, K, dx, dweight, dbias,
+    return status(dn_launch_linear_backward(type, dy, x, weight, z, M, N, K, activation, drop, dz_buffer, dx, dweight, dbias,
                                             static_cast<float *>(workspace), (hipStream_t)stream));
 }
 

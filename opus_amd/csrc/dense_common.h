@@ -255,6 +255,6 @@ hipError_t dn_launch_linear_forward(int type, const void *x, const void *w, cons
                                     long long M, long long N, long long K, int act, const DnDrop &drop, void *y,
                                     void *z, float *workspace, hipStream_t s);
 size_t dn_linear_backward_workspace(int type, long long M, long long N, long long K);
-hipError_t dn_launch_linear_backward(int type, const void *dz, const void *x, const void *w, long long M,
-                                     long long N, long long K, void *dx, void *dw, void *db, float *workspace,
-                                     hipStream_t s);
+hipError_t dn_launch_linear_backward(int type, const void *dy, const void *x, const void *w, const void *z, long long M,
+                                     long long N, long long K, int act, const DnDrop &drop, void *dz_buffer, void *dx,
+                                     void *dw, void *db, float *workspace, hipStream_t s);

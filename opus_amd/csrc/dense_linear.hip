@@ -84,7 +84,8 @@ struct GemmArgs {
     long long pitch;
     float *colsum;               // [splits * sharers][I]: shares of the sums over r of A(i, r) ..
     void *colsum_out;            // .. which belong here (at once, where there is one share); NULL: not wanted
-    int sharers;                 // tiles of a row of tiles that share the sums' work
+    int sharers;                 // tiles of a row of tiles that share the sums' work (0: `colsum` holds sums made before)
+    int sum_parts;               // rows of `colsum`
     Epilogue e;
 };
 
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(256) dense_gemm_join_kernel(JoinArgs a)
         block -= a.blocks[0];
     const GemmArgs &g = a.g[which];
     if (which && block >= a.blocks[1]) {
-        join_sums<T>(g.colsum, g.splits * g.sharers, g.I, static_cast<T *>(g.colsum_out), block - a.blocks[1]);
+        join_sums<T>(g.colsum, g.sum_parts, g.I, static_cast<T *>(g.colsum_out), block - a.blocks[1]);
         return;
     }
     const uint64_t seed = dn_seed(g.e.drop);
@@ -683,6 +684,49 @@ __global__ void __launch_bounds__(256) dense_colsum_kernel(const T *dz, long lon
     }
 }
 
+// dz = D(dy) act'(z), and its column sums before it is rounded to 16 bits (after that the sums would be off by 1.4 times
+// what their own rounding costs, 2 times where the kept elements' scale is half a step from a 16-bit number).  1 << lx
+// threads a row, eight columns each; 256 >> lx rows at a time, whose sums meet in LDS; a run of rows a workgroup, which
+// the kernels above add.
+struct DzArgs {
+    const void *dy, *z;
+    void *dz;
+    long long M, N, rows_per;
+    int lx, act;
+    DnDrop drop;
+    float *part;                 // [runs][N]
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a)
+{
+    __shared__ dn_floats<8> lds[256];
+    const int tid = threadIdx.x, x = tid & ((1 << a.lx) - 1), y = tid >> a.lx, lanes = 256 >> a.lx;
+    const long long col = (((long long)blockIdx.x << a.lx) + x) * 8, first = blockIdx.y * a.rows_per, last = min(first + a.rows_per, a.M);
+    const int n = (int)max(0ll, min(8ll, a.N - col));
+    const uint64_t seed = dn_seed(a.drop);
+    dn_floats<8> s = 0.f;
+    if (n > 0)
+        for (long long row = first + y; row < last; row += lanes) {
+            const long long at = row * a.N + col;
+            dn_floats<8> v = dn_load_n<8>(static_cast<const T *>(a.dy) + at, n, (int)a.N);
+            if (a.drop.threshold)
+                dn_drop<8>(v, row, (uint32_t)col, seed, a.drop);
+            if (a.z)
+                dn_act_slope<8>(v, dn_load_n<8>(static_cast<const T *>(a.z) + at, n, (int)a.N), a.act);
+            s += v;
+            dn_store_n<8>(static_cast<T *>(a.dz) + at, v, n);
+        }
+    lds[tid] = s;
+    for (int half = lanes >> 1; half; half >>= 1) {
+        __syncthreads();
+        if (y < half)
+            lds[tid] = s += lds[tid + (half << a.lx)];
+    }
+    if (y == 0)
+        dn_store_n<8>(a.part + blockIdx.y * a.N + col, s, n);
+}
+
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
@@ -791,7 +835,7 @@ Product product(const Plan &p, const void *a, const void *b, long long I, long l
     // (a tile's pieces are addressed in 32 bits from its corner)
     const auto near = [](bool rc, long long i, long long r) { return (rc ? 256 * r : 64 * i) * sizeof(T) < (1ll << 31); };
     return {{a, b, I, J, R, p.tiles_i, p.tiles_j, p.splits, p.steps, p.steps_per_split, p.splits > 1 ? shares : nullptr, p.pitch,
-             p.splits * p.sharers > 1 ? sums : nullptr, sums_out, p.sharers, e},
+             p.splits * p.sharers > 1 ? sums : nullptr, sums_out, p.sharers, p.splits * p.sharers, e},
             aligned16(a) && aligned16(b) && (ARC ? R : I) % piece == 0 && (BRC ? R : J) % piece == 0 && near(ARC, I, R) && near(BRC, J, R),
             (long long)p.tiles_i * p.tiles_j * p.splits};
 }
@@ -840,6 +884,22 @@ long long colsum_runs(long long M, long long N)
     return runs < 1 ? 1 : runs > 65535 ? 65535 : runs;
 }
 
+// dense_dz_kernel's threads a row (their logarithm), and its runs of rows: eight workgroups a CU, of two rows a thread or more
+int dz_lanes(long long N)
+{
+    int lx = 0;
+    while (lx < 5 && (8ll << lx) < N)
+        ++lx;
+    return lx;
+}
+long long dz_runs(long long M, long long N)
+{
+    const int lx = dz_lanes(N);
+    const long long want = dn_ceil(8 * CUS, dn_ceil(N, 8 << lx)), most = dn_ceil(M, 2 * (256 >> lx));
+    const long long runs = want < most ? want : most;
+    return runs < 1 ? 1 : runs;
+}
+
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // The backward's two products, as they are planned where both are wanted: side by side in one launch if their tiles
@@ -865,10 +925,19 @@ PlanPair plan_pair(int type, long long M, long long N, long long K)
 
 size_t sums_bytes(const Plan &p, long long N) { return (size_t)p.splits * p.sharers * N * sizeof(float); }
 
+// made: dz's column sums, [dz_runs][N], where they were made along with dz (else NULL)
 template <class T>
 hipError_t backward(int type, const void *dz, const void *x, const void *w, long long M, long long N, long long K,
-                    void *dx, void *dw, void *db, float *ws, hipStream_t s)
+                    void *dx, void *dw, void *db, float *ws, const float *made, hipStream_t s)
 {
+    const auto take = [&](Product q) {
+        if (made) {
+            q.g.colsum = const_cast<float *>(made);
+            q.g.sharers = 0;
+            q.g.sum_parts = (int)dz_runs(M, N);
+        }
+        return q;
+    };
     const bool want_dx = dx && M && K, want_dw = dw && N && K;
     const Epilogue ex = {nullptr, nullptr, dx, nullptr, OPUS_DENSE_ACT_NONE, {}}, ew = {nullptr, nullptr, dw, nullptr, OPUS_DENSE_ACT_NONE, {}};
     if (want_dx && want_dw) {
@@ -876,7 +945,7 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
         if (p.together) {
             float *const shares = ws + align256(p.dx.bytes) / sizeof(float), *const sums = shares + align256(p.dw.bytes) / sizeof(float);
             const Product qx = product<T, true, false>(p.dx, dz, w, M, K, N, ex, ws, nullptr, nullptr);
-            const Product qw = product<T, false, false>(p.dw, dz, x, N, K, M, ew, shares, sums, db);
+            const Product qw = take(product<T, false, false>(p.dw, dz, x, N, K, M, ew, shares, sums, db));
             const long long blocks = qx.blocks + qw.blocks;
             if (blocks * 256 > 0xFFFFFFFFll)
                 return hipErrorInvalidValue;
@@ -905,7 +974,10 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
     if (want_dw) {
         const Plan p = plan(type, N, K, M);
         float *const sums = ws + align256(p.bytes) / sizeof(float);
-        e = gemm<T, false, false>(p, product<T, false, false>(p, dz, x, N, K, M, ew, ws, sums, db), s);
+        e = gemm<T, false, false>(p, take(product<T, false, false>(p, dz, x, N, K, M, ew, ws, sums, db)), s);
+    } else if (db && N && made) {
+        hipLaunchKernelGGL(dense_colsum_join_kernel<T>, dim3((unsigned)dn_ceil(N, 16)), dim3(256), 0, s, made,
+                           (int)dz_runs(M, N), N, static_cast<T *>(db));
     } else if (db && N) {
         const long long runs = colsum_runs(M, N), per = dn_ceil(M > 0 ? M : 1, runs);
         hipLaunchKernelGGL(dense_colsum_kernel<T>, dim3((unsigned)dn_ceil(N, 32), (unsigned)runs), dim3(256), 0, s,
@@ -970,7 +1042,8 @@ hipError_t dn_launch_linear_forward(int type, const void *x, const void *w, cons
     return r != hipSuccess ? r : msmv_launch_status(stale);
 }
 
-size_t dn_linear_backward_workspace(int type, long long M, long long N, long long K)
+// the products' part of the backward's workspace; behind it, for 16-bit types, the column sums made along with dz
+static size_t products_workspace(int type, long long M, long long N, long long K)
 {
     if (N <= 0)
         return 0;
@@ -982,16 +1055,44 @@ size_t dn_linear_backward_workspace(int type, long long M, long long N, long lon
     at_least((size_t)colsum_runs(M, N) * N * sizeof(float));
     if (both.together)
         at_least(align256(both.dx.bytes) + align256(both.dw.bytes) + sums_bytes(both.dw, N));
-    return most;
+    return align256(most);
 }
 
-hipError_t dn_launch_linear_backward(int type, const void *dz, const void *x, const void *w, long long M,
-                                     long long N, long long K, void *dx, void *dw, void *db, float *workspace,
-                                     hipStream_t s)
+size_t dn_linear_backward_workspace(int type, long long M, long long N, long long K)
 {
+    if (N <= 0)
+        return 0;
+    const size_t products = products_workspace(type, M, N, K);
+    return type == OPUS_DENSE_F32 ? products : products + (size_t)dz_runs(M, N) * N * sizeof(float);
+}
+
+// The column sums are made along with dz only for 16-bit types: an fp32 dz is not rounded, and the products' workgroups
+// add it up at less cost.
+hipError_t dn_launch_linear_backward(int type, const void *dy, const void *x, const void *w, const void *z, long long M,
+                                     long long N, long long K, int act, const DnDrop &drop, void *dz_buffer, void *dx,
+                                     void *dw, void *db, float *workspace, hipStream_t s)
+{
+    const bool prepare = (act != OPUS_DENSE_ACT_NONE || drop.threshold) && M > 0 && N > 0;
+    float *made = nullptr;
+    hipError_t r = hipSuccess;
     const hipError_t stale = hipPeekAtLastError();
-    const hipError_t r = type == OPUS_DENSE_F32 ? backward<float>(type, dz, x, w, M, N, K, dx, dw, db, workspace, s)
-                       : type == OPUS_DENSE_BF16 ? backward<dn_bf16>(type, dz, x, w, M, N, K, dx, dw, db, workspace, s)
-                                                 : backward<dn_f16>(type, dz, x, w, M, N, K, dx, dw, db, workspace, s);
+    if (prepare && db && type != OPUS_DENSE_F32) {
+        made = workspace + products_workspace(type, M, N, K) / sizeof(float);
+        const long long runs = dz_runs(M, N);
+        const DzArgs a = {dy, act != OPUS_DENSE_ACT_NONE ? z : nullptr, dz_buffer, M, N, dn_ceil(M, runs), dz_lanes(N), act, drop, made};
+        const dim3 grid((unsigned)dn_ceil(N, 8 << a.lx), (unsigned)runs);
+        if (type == OPUS_DENSE_BF16)
+            hipLaunchKernelGGL(dense_dz_kernel<dn_bf16>, grid, dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL(dense_dz_kernel<dn_f16>, grid, dim3(256), 0, s, a);
+    } else if (prepare) {
+        r = dn_launch_elementwise(type, dy, nullptr, act != OPUS_DENSE_ACT_NONE ? z : nullptr, act, M, N, drop, dz_buffer, s);
+    }
+    if (r != hipSuccess)
+        return r;
+    const void *dz = prepare ? dz_buffer : dy;
+    r = type == OPUS_DENSE_F32 ? backward<float>(type, dz, x, w, M, N, K, dx, dw, db, workspace, made, s)
+      : type == OPUS_DENSE_BF16 ? backward<dn_bf16>(type, dz, x, w, M, N, K, dx, dw, db, workspace, made, s)
+                                : backward<dn_f16>(type, dz, x, w, M, N, K, dx, dw, db, workspace, made, s);
     return r != hipSuccess ? r : msmv_launch_status(stale);
 }

@@ -212,7 +212,7 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout_p=0.0
     "relu", "gelu" (with erf), "gelu_tanh" or "silu".  ``dropout_p``, ``seed``, ``offset``: see the module's text.
     Gradients flow to x, weight, bias and residual.  With an activation the backward needs x W^T + bias, which the
     forward then stores in the tensors' type (only where a gradient is wanted); d act(x W^T + bias) is rounded to that
-    type too before the two products of the backward."""
+    type too before the two products of the backward (the bias' gradient is summed before)."""
     _check("linear", x, ("weight", "bias", "residual"), (weight, bias, residual))
     shape, w_shape = x.shape, weight.shape
     if len(w_shape) != 2 or w_shape[1] != shape[-1]:

@@ -175,6 +175,23 @@ def test_linear_many_tiles(od, dtype):
     run_linear(od, 62, TYPES[dtype], 1031, 131, 1029, name="gelu")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,wants", [(512, 264, (True, True)), (300, 7, (True, True)), (512, 264, (False, False)), (77, 1003, (True, False)),
+                                       (4097, 40, (False, True)), (1, 24, (True, True))])
+def test_bias_gradient_is_summed_before_dz_is_rounded(od, dtype, m, n, wants):
+    """dy = 1 and a scale half a step from a 16-bit number: rounded first, dz and its sum would be off by half a step in
+    every column, beside the sum's own rounding.  Sums in fp32: m roundings at most."""
+    dtype = TYPES[dtype]
+    k = round(65536 * U[dtype]) - (dtype == torch.bfloat16)            # scale 1 + U, just below
+    x = torch.ones(m, 16, dtype=dtype, device="cuda", requires_grad=wants[0])
+    w = torch.ones(n, 16, dtype=dtype, device="cuda", requires_grad=wants[1])
+    b = torch.zeros(n, dtype=dtype, device="cuda", requires_grad=True)
+    y = od.linear(x, w, b, dropout_p=k / 65536, seed=9, offset=3)
+    y.backward(torch.ones_like(y))
+    want = do.keep(m, n, k / 65536, 9, 3).sum(0)
+    check(b.grad, want, rounded(want, dtype) + (m + 2) * 2.0 ** -24 * want, "dbias")
+
+
 @pytest.mark.parametrize("leave", ["x", "w", "b", "xw", "xb", "wb", "xwr"])
 def test_linear_gradients_asked_for_one_by_one(od, leave):
     run_linear(od, 70, torch.bfloat16, 150, 136, 72, name="silu", leave=tuple(leave))

@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(EW_THREADS) dense_elementwise_kernel(EwArgs a)
     if (a.drop.threshold)
         dn_drop<8>(v, row, col, seed, a.drop);
     if constexpr (SLOPE) {
-        dn_act_slope<8>(v, dn_load_n<8>(static_cast<const T *>(a.slope) + at, n, (int)a.cols), a.act);
+        dn_act_slope<8, T>(v, dn_load_n<8>(static_cast<const T *>(a.slope) + at, n, (int)a.cols), a.act);
     } else if (a.residual) {
         v += dn_load_n<8>(static_cast<const T *>(a.residual) + at, n, (int)a.cols);
     }

@@ -885,7 +885,8 @@ long long colsum_runs(long long M, long long N)
     return runs < 1 ? 1 : runs > 65535 ? 65535 : runs;
 }
 
-// dense_dz_kernel's threads a row (their logarithm), and its runs of rows: eight workgroups a CU, of two rows a thread or more
+// dense_dz_kernel's threads a row (their logarithm), and its runs of rows: eight workgroups a CU, of a row a thread or more
+// (1237 x 777 fp16: 7.5 us, of two rows 10.9)
 int dz_lanes(long long N)
 {
     int lx = 0;
@@ -896,7 +897,7 @@ int dz_lanes(long long N)
 long long dz_runs(long long M, long long N)
 {
     const int lx = dz_lanes(N);
-    const long long want = dn_ceil(8 * CUS, dn_ceil(N, 8 << lx)), most = dn_ceil(M, 2 * (256 >> lx));
+    const long long want = dn_ceil(8 * CUS, dn_ceil(N, 8 << lx)), most = dn_ceil(M, 256 >> lx);
     const long long runs = want < most ? want : most;
     return runs < 1 ? 1 : runs;
 }

@@ -13,7 +13,8 @@ statistics and the epilogue are in fp32 and every result is rounded once.  A ten
 first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep no
 state and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
 call on the same inputs gives the same bits (asking for other gradients along with one may round that one otherwise).
-Gradients are first-order only.
+Gradients are first-order only.  ``torch.jit.trace`` records the calls (not their backward, which raises); ``torch.fx``'s
+tracer at the dispatcher and ``torch.func``'s transforms are refused.
 
 ``D`` is dropout with a counter-based generator: whether element (row, column) is kept is computed from
 ``(seed, offset, row, column)`` - row counting the tensor's last-dimension rows - by Philox 4x32-10, in the forward
@@ -82,10 +83,10 @@ def _drop_struct(threshold, seed, offset):
     return _lib.DenseDropout(threshold, int(offset), int(seed) & (2 ** 64 - 1), None)
 
 
-def _seed_tensor(threshold, seed):
+def _seed_tensor(drop, seed):
     """The seed as what autograd keeps an eye on (None for a number): changed in place before the backward, it would
     give another mask there."""
-    return seed if threshold and isinstance(seed, torch.Tensor) else None
+    return seed if drop is not None and isinstance(seed, torch.Tensor) else None
 
 
 def _drop_again(drop, seed):
@@ -118,20 +119,45 @@ def _contiguous(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _wants_grad(tensors):
+def _refuse_transforms(what, tensors):
+    """A graph tracer at the dispatcher (make_fx) and functionalisation see the allocations of a call but not its kernels:
+    what they make of it would return memory nobody wrote."""
+    if _dispatch_modes() or torch._ops._len_torch_dispatch_stack_pre_dispatch():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is not None:
+            raise RuntimeError(f"{what}: cannot be traced by torch.fx")
+    if _transforms_active() and any(t is not None and torch._is_functional_tensor(t) for t in tensors):
+        raise RuntimeError(f"{what}: cannot be functionalised")
+
+
+_tracing_state = torch._C._get_tracing_state
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_transforms_active = torch._C._are_functorch_transforms_active
+
+
+def _needs_autograd(what, tensors):
+    """Whether a call has to go through its autograd function: where a gradient is wanted, and under ``torch.jit.trace``,
+    which records that function and not the kernels inside."""
+    _refuse_transforms(what, tensors)
+    if _tracing_state() is not None:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if t is not None and getattr(t, "requires_grad", False):        # (what is no tensor is refused later)
                 return True
     return False
 
 
 def _first_order(backward):
-    """``once_differentiable``, entered only where a graph of the backward is asked for."""
+    """``once_differentiable``, entered only where a graph of the backward is asked for; other ways to look into the
+    backward are refused."""
     guarded = once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        _refuse_transforms("backward", grads)
+        if _tracing_state() is not None:
+            raise RuntimeError("a backward of a dense operator cannot be traced")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return staticmethod(run)
 
@@ -155,27 +181,40 @@ def _norm_backward_workspace(kind, rows, width, gate_rows):
 # ------------------------------------------------------------------------------------------------
 # linear
 # ------------------------------------------------------------------------------------------------
-def _linear_forward(x, weight, bias, residual, activation, drop, want_z):
-    N, K = weight.shape
+def _linear_forward(x, weight, bias, residual, activation, dropout_p, seed, offset, want_z):
+    """-> y, z or None, the activation's code, the dropout.  The checks are here, so that a traced call makes them too."""
+    _check("linear", x, ("weight", "bias", "residual"), (weight, bias, residual))
+    shape, w_shape = x.shape, weight.shape
+    if len(w_shape) != 2 or w_shape[1] != shape[-1]:
+        raise RuntimeError(f"linear: weight {list(w_shape)} does not fit x {list(shape)}")
+    if bias is not None and bias.shape != w_shape[:1]:
+        raise RuntimeError(f"linear: bias {list(bias.shape)} does not fit weight {list(w_shape)}")
+    if residual is not None and residual.shape != shape[:-1] + w_shape[:1]:
+        raise RuntimeError(f"linear: residual {list(residual.shape)} is not of the output's shape")
+    code = _lib.DENSE_ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"linear: activation has to be one of {sorted(_lib.DENSE_ACTIVATIONS)}, got {activation!r}")
+    threshold = _threshold("linear", dropout_p, seed, offset, x.device) if dropout_p != 0.0 else 0
+    drop = _drop_struct(threshold, seed, offset)
+    N, K = w_shape
     x, weight, bias, residual = _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual)
     kind, device = _TYPES[x.dtype], x.device
-    y = x.new_empty(x.shape[:-1] + (N,))
+    y = x.new_empty(shape[:-1] + w_shape[:1])
     M = x.numel() // K if K else y.numel() // max(N, 1)
-    z = torch.empty_like(y) if want_z else None
+    z = torch.empty_like(y) if want_z and code else None
     need = _linear_workspace(kind, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _run("linear", _lib.load().opus_dense_linear_forward, device, kind, x.data_ptr(), weight.data_ptr(), _ptr(bias),
-         _ptr(residual), M, N, K, activation, drop, y.data_ptr(), _ptr(z), _ptr(ws), need)
-    return y, z
+         _ptr(residual), M, N, K, code, drop, y.data_ptr(), _ptr(z), _ptr(ws), need)
+    return y, z, code, drop
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, threshold, seed, offset):
-        drop = _drop_struct(threshold, seed, offset)
-        y, z = _linear_forward(x, weight, bias, residual, activation, drop, activation != 0)
-        ctx.save_for_backward(x, weight, z, _seed_tensor(threshold, seed))
-        ctx.settings = activation, drop
+    def forward(ctx, x, weight, bias, residual, activation, dropout_p, seed, offset):
+        y, z, code, drop = _linear_forward(x, weight, bias, residual, activation, dropout_p, seed, offset, True)
+        ctx.save_for_backward(x, weight, z, _seed_tensor(drop, seed))
+        ctx.settings = code, drop
         return y
 
     @_first_order
@@ -213,21 +252,10 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout_p=0.0
     Gradients flow to x, weight, bias and residual.  With an activation the backward needs x W^T + bias, which the
     forward then stores in the tensors' type (only where a gradient is wanted); d act(x W^T + bias) is rounded to that
     type too before the two products of the backward (the bias' gradient is summed before)."""
-    _check("linear", x, ("weight", "bias", "residual"), (weight, bias, residual))
-    shape, w_shape = x.shape, weight.shape
-    if len(w_shape) != 2 or w_shape[1] != shape[-1]:
-        raise RuntimeError(f"linear: weight {list(w_shape)} does not fit x {list(shape)}")
-    if bias is not None and bias.shape != w_shape[:1]:
-        raise RuntimeError(f"linear: bias {list(bias.shape)} does not fit weight {list(w_shape)}")
-    if residual is not None and residual.shape != shape[:-1] + w_shape[:1]:
-        raise RuntimeError(f"linear: residual {list(residual.shape)} is not of the output's shape")
-    code = _lib.DENSE_ACTIVATIONS.get(activation)
-    if code is None:
-        raise ValueError(f"linear: activation has to be one of {sorted(_lib.DENSE_ACTIVATIONS)}, got {activation!r}")
-    threshold = _threshold("linear", dropout_p, seed, offset, x.device) if dropout_p != 0.0 else 0
-    if _wants_grad((x, weight, bias, residual)):
-        return _Linear.apply(x, weight, bias, residual, code, threshold, seed, offset)
-    return _linear_forward(x, weight, bias, residual, code, _drop_struct(threshold, seed, offset), False)[0]
+    args = x, weight, bias, residual, activation, dropout_p, seed, offset
+    if _needs_autograd("linear", args[:4]):
+        return _Linear.apply(*args)
+    return _linear_forward(*args, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------
@@ -238,52 +266,6 @@ def _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop):
     return _lib.DenseNorm(_TYPES[x.dtype], kind, rows, x.shape[-1], gate_rows, eps, scale, x.data_ptr(),
                           block.data_ptr(), _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
                           None if drop is None else ctypes.addressof(drop))
-
-
-def _norm_forward(tensors, kind, gate_rows, eps, scale, drop, want_stream, want_stats):
-    tensors = [_contiguous(t) for t in tensors]
-    x = tensors[0]
-    rows = x.numel() // x.shape[-1]
-    y = torch.empty_like(x)
-    stream = torch.empty_like(x) if want_stream else None
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
-    args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop)
-    _run("residual_norm", _lib.load().opus_dense_norm_forward, x.device, args, y.data_ptr(), _ptr(stream), _ptr(stats))
-    return y, stream, stats
-
-
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, block, weight, bias, post_weight, post_bias, gate, settings):
-        kind, gate_rows, eps, scale, threshold, seed, offset, want_stream = settings
-        tensors = (x, block, weight, bias, post_weight, post_bias, gate)
-        drop = _drop_struct(threshold, seed, offset)
-        y, stream, stats = _norm_forward(tensors, kind, gate_rows, eps, scale, drop, want_stream, True)
-        ctx.save_for_backward(*tensors, stats, _seed_tensor(threshold, seed))
-        ctx.settings = kind, gate_rows, eps, scale, drop
-        ctx.set_materialize_grads(False)
-        return (y, stream) if want_stream else y
-
-    @_first_order
-    def backward(ctx, dy, dstream=None):
-        if dy is None and dstream is None:
-            return (None,) * 8
-        saved = ctx.saved_tensors
-        kind, gate_rows, eps, scale, drop = ctx.settings
-        drop = _drop_again(drop, saved[8])
-        tensors, stats = [_contiguous(t) for t in saved[:7]], saved[7]
-        grads = [torch.empty_like(t) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
-        x = tensors[0]
-        width = x.shape[-1]
-        rows = x.numel() // width
-        dy, dstream = _contiguous(dy), _contiguous(dstream)
-        args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop)
-        need = _norm_backward_workspace(args.type, rows, width, gate_rows)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        _run("residual_norm backward", _lib.load().opus_dense_norm_backward, x.device, args, _ptr(dy), _ptr(dstream),
-             stats.data_ptr(), _lib.DenseNormGrads(*[None if g is None else g.data_ptr() for g in grads]), _ptr(ws),
-             need)
-        return (*grads, None)
 
 
 _NORM_NAMES = ("block", "weight", "bias", "post_weight", "post_bias", "gate")
@@ -309,22 +291,9 @@ def _gate_rows(x, gate):
                        f"trailing leading dimensions")
 
 
-def residual_norm(x, block, weight=None, bias=None, kind="layer", eps=1e-5, post_weight=None, post_bias=None, gate=None,
-                  residual_scale=1.0, dropout_p=0.0, seed=None, offset=0, return_stream=False):
-    """The norm between two blocks, with what joins the first block's output to the stream.
-
-        r = residual_scale * x + gate * D(post(block));  y = norm(r)
-
-    x and block [..., width], width at most 16384.  ``kind``: "layer" (mean and variance) or "rms" (mean square), for
-    both norms; ``eps`` is added to the variance (mean square).  weight, bias [width] or None (1 and 0).
-    ``post_weight`` [width] puts a norm of the block's output before the sum (``post_bias`` [width] or None); None:
-    the block's output enters as it is.  ``gate``: [width], one row for each index of x's first dimension
-    ([x.shape[0], width]), one for each row (x's shape), or x's shape with ones in place of its last leading
-    dimensions; None: 1.  ``residual_scale`` is a number.  ``dropout_p``, ``seed``, ``offset``: see the module's text.
-
-    Returns y, or (y, r) with ``return_stream``.  y is computed from the unrounded r.  Gradients flow to all tensors,
-    from either result; the backward computes r again from x and block, so that only two statistics for each norm
-    and row are kept."""
+def _norm_forward(x, block, weight, bias, post_weight, post_bias, gate, kind, eps, residual_scale, dropout_p, seed, offset,
+                  want_stream, want_stats):
+    """-> y, r or None, the statistics or None, the settings.  The checks are here, so that a traced call makes them too."""
     tensors = (x, block, weight, bias, post_weight, post_bias, gate)
     _check("residual_norm", x, _NORM_NAMES, tensors[1:])
     shape = x.shape
@@ -349,11 +318,72 @@ def residual_norm(x, block, weight=None, bias=None, kind="layer", eps=1e-5, post
         raise ValueError(f"residual_norm: eps has to be no less than 0, got {eps}")
     gate_rows = 0 if gate is None else _gate_rows(x, gate)
     threshold = _threshold("residual_norm", dropout_p, seed, offset, x.device) if dropout_p != 0.0 else 0
-    if _wants_grad(tensors):
-        return _ResidualNorm.apply(*tensors, (code, gate_rows, eps, residual_scale, threshold, seed, offset,
-                                              return_stream))
-    y, stream, _ = _norm_forward(tensors, code, gate_rows, eps, residual_scale, _drop_struct(threshold, seed, offset),
-                                 return_stream, False)
+    drop = _drop_struct(threshold, seed, offset)
+    tensors = [_contiguous(t) for t in tensors]
+    x = tensors[0]
+    rows = x.numel() // width
+    y = torch.empty_like(x)
+    stream = torch.empty_like(x) if want_stream else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
+    args = _norm_struct(tensors, code, rows, gate_rows, eps, residual_scale, drop)
+    _run("residual_norm", _lib.load().opus_dense_norm_forward, x.device, args, y.data_ptr(), _ptr(stream), _ptr(stats))
+    return y, stream, stats, (code, gate_rows, eps, residual_scale, drop)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, block, weight, bias, post_weight, post_bias, gate, kind, eps, residual_scale, dropout_p, seed, offset,
+                want_stream):
+        tensors = (x, block, weight, bias, post_weight, post_bias, gate)
+        y, stream, stats, ctx.settings = _norm_forward(*tensors, kind, eps, residual_scale, dropout_p, seed, offset,
+                                                       want_stream, True)
+        ctx.save_for_backward(*tensors, stats, _seed_tensor(ctx.settings[4], seed))
+        ctx.set_materialize_grads(False)
+        return (y, stream) if want_stream else y
+
+    @_first_order
+    def backward(ctx, dy, dstream=None):
+        if dy is None and dstream is None:
+            return (None,) * 14
+        saved = ctx.saved_tensors
+        kind, gate_rows, eps, scale, drop = ctx.settings
+        drop = _drop_again(drop, saved[8])
+        tensors, stats = [_contiguous(t) for t in saved[:7]], saved[7]
+        grads = [torch.empty_like(t) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
+        x = tensors[0]
+        width = x.shape[-1]
+        rows = x.numel() // width
+        dy, dstream = _contiguous(dy), _contiguous(dstream)
+        args = _norm_struct(tensors, kind, rows, gate_rows, eps, scale, drop)
+        need = _norm_backward_workspace(args.type, rows, width, gate_rows)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        _run("residual_norm backward", _lib.load().opus_dense_norm_backward, x.device, args, _ptr(dy), _ptr(dstream),
+             stats.data_ptr(), _lib.DenseNormGrads(*[None if g is None else g.data_ptr() for g in grads]), _ptr(ws),
+             need)
+        return (*grads, *(None,) * 7)
+
+
+def residual_norm(x, block, weight=None, bias=None, kind="layer", eps=1e-5, post_weight=None, post_bias=None, gate=None,
+                  residual_scale=1.0, dropout_p=0.0, seed=None, offset=0, return_stream=False):
+    """The norm between two blocks, with what joins the first block's output to the stream.
+
+        r = residual_scale * x + gate * D(post(block));  y = norm(r)
+
+    x and block [..., width], width at most 16384.  ``kind``: "layer" (mean and variance) or "rms" (mean square), for
+    both norms; ``eps`` is added to the variance (mean square).  weight, bias [width] or None (1 and 0).
+    ``post_weight`` [width] puts a norm of the block's output before the sum (``post_bias`` [width] or None); None:
+    the block's output enters as it is.  ``gate``: [width], one row for each index of x's first dimension
+    ([x.shape[0], width]), one for each row (x's shape), or x's shape with ones in place of its last leading
+    dimensions; None: 1.  ``residual_scale`` is a number.  ``dropout_p``, ``seed``, ``offset``: see the module's text.
+
+    Returns y, or (y, r) with ``return_stream``.  y is computed from the unrounded r.  Gradients flow to all tensors,
+    from either result; the backward computes r again from x and block, so that only two statistics for each norm
+    and row are kept."""
+    args = (x, block, weight, bias, post_weight, post_bias, gate, kind, eps, residual_scale, dropout_p, seed, offset,
+            return_stream)
+    if _needs_autograd("residual_norm", args[:7]):
+        return _ResidualNorm.apply(*args)
+    y, stream, _, _ = _norm_forward(*args, False)
     return (y, stream) if return_stream else y
 
 
@@ -369,14 +399,23 @@ def _dropout(x, residual, drop):
     return y
 
 
+def _dropout_forward(x, residual, p, seed, offset):
+    """-> y, the dropout.  The checks are here, so that a traced call makes them too."""
+    _check("dropout", x, ("residual",), (residual,))
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"dropout: residual {list(residual.shape)} is not of x's shape {list(x.shape)}")
+    drop = _drop_struct(_threshold("dropout", p, seed, offset, x.device), seed, offset)
+    return _dropout(x, residual, drop), drop
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, threshold, seed, offset):
-        ctx.drop = _drop_struct(threshold, seed, offset)
-        watched = _seed_tensor(threshold, seed)
+    def forward(ctx, x, residual, p, seed, offset):
+        y, ctx.drop = _dropout_forward(x, residual, p, seed, offset)
+        watched = _seed_tensor(ctx.drop, seed)
         if watched is not None:
             ctx.save_for_backward(watched)
-        return _dropout(x, residual, ctx.drop)
+        return y
 
     @_first_order
     def backward(ctx, dy):
@@ -389,10 +428,6 @@ class _Dropout(torch.autograd.Function):
 def dropout(x, p, seed, offset=0, residual=None):
     """``residual + D(x)``: x [..., columns], residual of x's shape or None.  See the module's text for ``D``.
     Gradients flow to x and residual."""
-    _check("dropout", x, ("residual",), (residual,))
-    if residual is not None and residual.shape != x.shape:
-        raise RuntimeError(f"dropout: residual {list(residual.shape)} is not of x's shape {list(x.shape)}")
-    threshold = _threshold("dropout", p, seed, offset, x.device)
-    if _wants_grad((x, residual)):
-        return _Dropout.apply(x, residual, threshold, seed, offset)
-    return _dropout(x, residual, _drop_struct(threshold, seed, offset))
+    if _needs_autograd("dropout", (x, residual)):
+        return _Dropout.apply(x, residual, p, seed, offset)
+    return _dropout_forward(x, residual, p, seed, offset)[0]

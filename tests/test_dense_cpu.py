@@ -247,3 +247,105 @@ def test_oracle_norm_gradients_against_differences(kind, post):
             down = loss()
             arr[i] = old
             assert abs((up - down) / (2 * h) - out["d" + name][i]) < 1e-7, name
+
+
+# ------------------------------------------------------------------------------------------------
+# tracers and transforms, with C entries of the library's own signatures that work on host memory
+# ------------------------------------------------------------------------------------------------
+@pytest.fixture
+def standin(monkeypatch, lib):
+    """opus_dense on CPU tensors: y = x W^T (+ the dropout's offset), y = x + block and r = 2 y, y = 2 x (+ the seed)."""
+    from opus_amd import _lib, opus_dense as od
+
+    def array(p, *shape):
+        return np.ctypeslib.as_array((ctypes.c_float * int(np.prod(shape))).from_address(p)).reshape(shape)
+
+    def linear(kind, x, w, b, r, M, N, K, act, drop, y, z, ws, need, stream):
+        array(y, M, N)[:] = array(x, M, K) @ array(w, N, K).T + (drop.contents.offset if drop else 0)
+        return 0
+
+    def norm(s, y, stream_out, stats, stream):
+        s = s.contents
+        array(y, s.rows, s.width)[:] = array(s.x, s.rows, s.width) + array(s.block, s.rows, s.width)
+        if stream_out:
+            array(stream_out, s.rows, s.width)[:] = 2 * array(y, s.rows, s.width)
+        return 0
+
+    def dropout(kind, x, r, rows, cols, drop, y, stream):
+        seed = ctypes.c_longlong.from_address(drop.contents.seed_ptr).value if drop.contents.seed_ptr else drop.contents.seed
+        array(y, rows, cols)[:] = 2 * array(x, rows, cols) + seed
+        return 0
+
+    class Library:
+        pass
+
+    entries = {"opus_dense_linear_forward": linear, "opus_dense_norm_forward": norm, "opus_dense_dropout": dropout}
+    for name, (result, arguments) in _lib.DENSE_SYMBOLS.items():
+        f = entries.get(name)
+        setattr(Library, name, staticmethod(ctypes.CFUNCTYPE(result, *arguments)(f) if f else getattr(lib, name)))
+    monkeypatch.setattr(_lib, "load", lambda: Library)
+    monkeypatch.setattr(od, "_check", lambda *a: None)
+    monkeypatch.setattr(od, "_run", lambda what, fn, device, *args: _lib.check_dense(fn(*args, None), what))
+    return od
+
+
+W = torch.arange(18.0).view(3, 6) - 8
+CALLS = {
+    "linear": lambda od, x: od.linear(x, W),
+    "linear, everything": lambda od, x: od.linear(x, W, torch.ones(3), "gelu", torch.ones(*x.shape[:-1], 3), 0.5, 3, 7),
+    "norm": lambda od, x: od.residual_norm(x, x),
+    "norm's stream": lambda od, x: od.residual_norm(x, x, gate=x, return_stream=True)[1],
+    "dropout": lambda od, x: od.dropout(x, 0.5, 5),
+}
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("wants_grad", [False, True])
+@pytest.mark.parametrize("enabled", [False, True])
+def test_a_traced_call_runs_its_kernel(standin, name, wants_grad, enabled):
+    """The traced module computes, for other values and another number of rows too; it does not hand out memory that was
+    only allocated."""
+    f = lambda x: CALLS[name](standin, x)                                       # noqa: E731
+    with torch.set_grad_enabled(enabled):
+        traced = torch.jit.trace(f, (torch.randn(4, 6, requires_grad=wants_grad),), check_trace=False)
+        for rows in (4, 9):
+            x = torch.randn(rows, 6)
+            held = [torch.full((rows, c), 7.0) for c in (3, 6) for _ in range(20)]
+            del held                                                            # (what fresh memory may hold)
+            assert torch.equal(traced(x).detach(), f(x))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_a_traced_call_reads_its_seed_tensor_and_checks_its_arguments(standin):
+    traced = torch.jit.trace(lambda x, s: standin.dropout(x, 0.5, s), (torch.zeros(2, 3), torch.tensor([4])), check_trace=False)
+    assert (traced(torch.zeros(2, 3), torch.tensor([9])) == 9).all()
+    traced = torch.jit.trace(lambda x, w: standin.linear(x, w), (torch.zeros(2, 6), W), check_trace=False)
+    with pytest.raises(RuntimeError, match="does not fit x"):
+        traced(torch.zeros(2, 6), torch.zeros(3, 5))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_other_transforms_are_refused(standin, name):
+    """An error instead of a result without the kernels' work."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x = lambda x: CALLS[name](standin, x), torch.randn(4, 6)                 # noqa: E731
+    want = f(x)
+    for call in (make_fx(f), make_fx(f, pre_dispatch=True), make_fx(f, tracing_mode="fake"), torch.func.functionalize(f),
+                 torch.func.vmap(f), torch.func.grad(lambda v: f(v).sum()), lambda v: torch.func.jvp(f, (v,), (v,))):
+        with pytest.raises(RuntimeError):
+            call(x)
+    assert torch.equal(f(x), want)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", CALLS)
+def test_a_traced_backward_is_refused(standin, name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(4, 6, requires_grad=True)
+    y = CALLS[name](standin, x)
+    dy = torch.ones_like(y)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda g: torch.autograd.grad(y, x, g)[0])(dy)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda v: torch.autograd.grad(CALLS[name](standin, v).sum(), v)[0], (x,), check_trace=False)

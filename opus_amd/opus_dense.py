@@ -13,8 +13,9 @@ statistics and the epilogue are in fp32 and every result is rounded once.  A ten
 first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep no
 state and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
 call on the same inputs gives the same bits (asking for other gradients along with one may round that one otherwise).
-Gradients are first-order only.  ``torch.jit.trace`` records the calls (not their backward, which raises); ``torch.fx``'s
-tracer at the dispatcher and ``torch.func``'s transforms are refused.
+Gradients are first-order and reverse-mode only: a tensor with a forward-mode tangent is refused, before or in a backward.
+``torch.jit.trace`` records the calls (not their backward, which raises); ``torch.fx``'s tracer at the dispatcher and
+``torch.func``'s transforms are refused.
 
 ``D`` is dropout with a counter-based generator: whether element (row, column) is kept is computed from
 ``(seed, offset, row, column)`` - row counting the tensor's last-dimension rows - by Philox 4x32-10, in the forward
@@ -29,6 +30,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -136,10 +138,11 @@ _transforms_active = torch._C._are_functorch_transforms_active
 
 
 def _needs_autograd(what, tensors):
-    """Whether a call has to go through its autograd function: where a gradient is wanted, and under ``torch.jit.trace``,
-    which records that function and not the kernels inside."""
+    """Whether a call has to go through its autograd function: where a gradient is wanted; under ``torch.jit.trace``, which
+    records that function and not the kernels inside; and in a forward-mode level, where that function refuses a tensor
+    with a tangent, which would otherwise be lost."""
     _refuse_transforms(what, tensors)
-    if _tracing_state() is not None:
+    if _tracing_state() is not None or forward_ad._current_level >= 0:
         return True
     if torch.is_grad_enabled():
         for t in tensors:
@@ -158,6 +161,8 @@ def _first_order(backward):
         _refuse_transforms("backward", grads)
         if _tracing_state() is not None:
             raise RuntimeError("a backward of a dense operator cannot be traced")
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise RuntimeError("gradients of a dense operator are first-order only: no tangent goes through its backward")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return staticmethod(run)
 

@@ -349,3 +349,22 @@ def test_a_traced_backward_is_refused(standin, name):
         make_fx(lambda g: torch.autograd.grad(y, x, g)[0])(dy)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(lambda v: torch.autograd.grad(CALLS[name](standin, v).sum(), v)[0], (x,), check_trace=False)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_tangent_is_refused(standin, name):
+    """Without a jvp the result would have no tangent, which reads as a derivative of zero."""
+    from torch.autograd import forward_ad
+    f, x = lambda x: CALLS[name](standin, x), torch.randn(4, 6)                 # noqa: E731
+    want = f(x)
+    with forward_ad.dual_level():
+        assert torch.equal(f(x), want)                                          # no tangent, nothing to lose
+        for primal in (x, x.clone().requires_grad_(True)):
+            dual = forward_ad.make_dual(primal, torch.ones_like(x))
+            for enabled in (True, False):
+                with torch.set_grad_enabled(enabled), pytest.raises(NotImplementedError):
+                    f(dual)
+        leaf = x.clone().requires_grad_(True)
+        y = f(leaf)
+        with pytest.raises(RuntimeError, match="no tangent goes through"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))

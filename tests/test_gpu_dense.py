@@ -827,3 +827,25 @@ def test_offsets_beyond_32_bits(od):
     d = od.dropout(x, 0.5, 9)
     k = torch.from_numpy(do.keep(5, width, 0.5, 9, first_row=rows - 5)).cuda()
     assert torch.equal(d[-5:].double(), x[-5:].double() * k)
+
+
+def test_tangents_are_refused_and_traced_calls_compute(od):
+    """A tangent raises instead of being lost, in the backward's own thread too; a traced module runs the kernels."""
+    import warnings
+    from torch.autograd import forward_ad
+    x, w = torch.randn(4, 16, device="cuda"), torch.randn(16, 16, device="cuda")
+    for f in (lambda x: od.linear(x, w, activation="gelu"), lambda x: od.residual_norm(x, x, gate=x), lambda x: od.dropout(x, 0.5, 3)):
+        want, other = f(x), torch.randn(7, 16, device="cuda")
+        with forward_ad.dual_level():
+            assert torch.equal(f(x), want)
+            with pytest.raises(NotImplementedError):
+                f(forward_ad.make_dual(x, x))
+            leaf = x.clone().requires_grad_(True)
+            with pytest.raises(RuntimeError, match="no tangent goes through"):
+                torch.autograd.grad(f(leaf), leaf, forward_ad.make_dual(want, want))
+        with warnings.catch_warnings():
+            warnings.simplefilter("ignore")
+            traced = torch.jit.trace(f, (x,), check_trace=False)
+        held = [torch.full((7, 16), 7.0, device="cuda") for _ in range(20)]
+        del held
+        assert torch.equal(traced(other), f(other)) and torch.equal(traced(x), want)

@@ -57,12 +57,21 @@ __device__ __forceinline__ void finish(const Epilogue &e, dn_floats<8> v, const 
     v += bias;
     if (e.z) {
         dn_floats<8> z = v;
-        // fp16: a tiny z must not become 0, or relu's gradient would take it for a negative one
-        if constexpr (sizeof(T) == 2)
+        // What the rounding to 16 bits must not do: make a tiny z 0, which relu's gradient would take for a negative one, or a
+        // large finite one inf, whose slope under gelu or silu would be inf x 0.
+        if constexpr (sizeof(T) == 2) {
+            constexpr float MOST = __is_same(T, dn_f16) ? 65504.f : 0x1.FEp127f;
+            if (e.act == OPUS_DENSE_ACT_RELU) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if ((float)(T)z[j] == 0.f && z[j] > 0.f)
-                    z[j] = 6e-8f;
+                for (int j = 0; j < 8; ++j)
+                    if ((float)(T)z[j] == 0.f && z[j] > 0.f)
+                        z[j] = 6e-8f;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    z[j] = __builtin_isinf(z[j]) || z[j] != z[j] ? z[j] : __builtin_amdgcn_fmed3f(z[j], -MOST, MOST);
+            }
+        }
         dn_store_n<8>(static_cast<T *>(e.z) + at, z, n);
     }
     dn_act<8, T>(v, e.act);

@@ -849,3 +849,46 @@ def test_tangents_are_refused_and_traced_calls_compute(od):
         held = [torch.full((7, 16), 7.0, device="cuda") for _ in range(20)]
         del held
         assert torch.equal(traced(other), f(other)) and torch.equal(traced(x), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("M,K,N", [(5, 24, 40), (70, 40, 72), (40, 4096, 64), (300, 33, 260)])
+def test_linear_gradients_where_x_w_is_beyond_the_type(od, dtype, name, M, K, N):
+    """z larger than the type's largest number, which the forward keeps for the backward: slopes are 0 or 1 there, never NaN.
+    z = x[m, 0] w[n, 0] is exact in fp32 (the other columns of x are 0), so its own error is the rounding where it is kept
+    (eslope as in linear_bounds, up to |z| = 64; beyond, the slopes are 0 or 1 but for 64 exp(-64))."""
+    dtype = TYPES[dtype]
+    rng = np.random.default_rng(M)
+    # fp16: up to 1e6; bf16: 181^2 2^113 = 1.9996 x 2^127, which rounds to inf in bf16 and not in fp32
+    big = (1000.0, 1000.0) if dtype == torch.float16 else (181 * 2.0 ** 56, 181 * 2.0 ** 57)
+    x, w = torch.zeros(M, K), torch.from_numpy(rng.standard_normal((N, K))).float()
+    x[:, 0] = torch.from_numpy(rng.choice([-1.0, 1.0], M) * rng.choice([0.001, 0.5, 1, big[0]], M))
+    w[:, 0] = torch.from_numpy(rng.choice([-1.0, 1.0], N) * rng.choice([0.25, 1, big[1]], N))
+    x, w = x.to(dtype).cuda().requires_grad_(True), w.to(dtype).cuda().requires_grad_(True)
+    b = torch.zeros(N, dtype=dtype, device="cuda", requires_grad=True)
+    dy, p = make(rng, dtype, M, N, std=0.01), 0.3
+    kept = do.keep(M, N, p, 77, 5)
+    with np.errstate(over="ignore"):
+        value, z = do.linear(f64(x), f64(w), None, name)
+        slope = do.act(z, name)[1]
+    far = np.abs(z) > torch.finfo(dtype).max
+    assert far.any() and not far.all() and np.abs(z).max() < torch.finfo(torch.float32).max
+    slope = np.where(np.abs(z) > 64, (z > 0).astype(float), slope)
+    y = od.linear(x, w, b, activation=name, dropout_p=p, seed=77, offset=5)
+    low = (z < 0) | (np.abs(z) < 64)                             # where y is small enough for the type too
+    value = np.where(low, value * kept, 0.0)
+    value = np.where(np.abs(z) > 64, 0.0, value)
+    got = np.where(low, f64(y), 0.0)
+    assert (np.abs(got - value) <= kept * 2.0 ** -19 * (np.abs(z) * low * (np.abs(z) < 64) + 1) + rounded(value, dtype)).all()
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], dy)
+    dz = f64(dy) * kept * slope
+    eslope = np.where(np.abs(z) > 64, 0.0, 0.8 * (U[dtype] * np.abs(z) + TINY[dtype]) + 32 * STEP * (1 + np.abs(z))) * (name != "relu")
+    edz = np.abs(f64(dy)) * kept * (eslope + 4 * STEP)
+    edz = edz + rounded(np.abs(dz) + edz, dtype)
+    a = np.abs(dz) + edz
+    for n, g, want, e, sums in (("dx", gx, dz @ f64(w), edz @ np.abs(f64(w)), a @ np.abs(f64(w)) * (N + 2)),
+                                ("dw", gw, dz.T @ f64(x), edz.T @ np.abs(f64(x)), a.T @ np.abs(f64(x)) * (M + 2)),
+                                ("db", gb, dz.sum(0), edz.sum(0), a.sum(0) * (M + 2))):
+        e = e + STEP * sums
+        check(g, want, e * (1 + U[dtype]) + rounded(want, dtype), f"{dtype} M{M} K{K} N{N} {name} {n}")

@@ -3,7 +3,7 @@ import math
 
 import numpy as np
 
-_ERF = np.frompyfunc(math.erf, 1, 1)
+_ERFC = np.frompyfunc(math.erfc, 1, 1)
 
 
 def philox(counter, key, rounds=10):
@@ -46,7 +46,7 @@ def act(z, name):
         s = 1 / (1 + np.exp(-z))
         return z * s, s * (1 + z * (1 - s))
     if name == "gelu":
-        cdf = 0.5 * (1 + _ERF(z / math.sqrt(2)).astype(np.float64))
+        cdf = 0.5 * _ERFC(-z / math.sqrt(2)).astype(np.float64)
         return z * cdf, cdf + z * np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     c = math.sqrt(2 / math.pi)
     t = np.tanh(c * (z + 0.044715 * z ** 3))

@@ -3,6 +3,8 @@
 Tolerances are bounds, element by element, from the arithmetic: U[t] = eps / 2 of the output's type for its one
 rounding (plus half the smallest subnormal), and 2^-23 a step of an fp32 sum (a rounding of 2^-24, and as much again
 for what a matrix instruction may drop inside) times the sum of the terms' magnitudes."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -892,3 +894,25 @@ def test_linear_gradients_where_x_w_is_beyond_the_type(od, dtype, name, M, K, N)
                                 ("db", gb, dz.sum(0), edz.sum(0), a.sum(0) * (M + 2))):
         e = e + STEP * sums
         check(g, want, e * (1 + U[dtype]) + rounded(want, dtype), f"{dtype} M{M} K{K} N{N} {name} {n}")
+
+
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES)
+def test_gelu_keeps_its_tail(od, dtype):
+    """Relative to the value: z Phi(z) = z erfc(-z / sqrt 2) / 2, far below where 1 + erf is 0 in fp32.  The argument's two
+    roundings change erfc by (z^2 + |z|) of it each, erfc itself is good to a few steps: 2^-21 (1 + z^2) of the value; below
+    2^-126 of erfc or of exp(-z^2 / 2) what is left may become 0 (times |z| < 16)."""
+    if dtype == torch.float32:
+        x = torch.linspace(-15, 15, 60001)
+    else:
+        x = torch.arange(-2 ** 15, 2 ** 15).to(torch.int16).view(dtype)
+        x = x[x.abs() <= 15]
+    x = x.reshape(-1, 1).cuda().requires_grad_()
+    z = f64(x)
+    cdf = 0.5 * np.array([math.erfc(-v / math.sqrt(2)) for v in z.ravel()]).reshape(z.shape)
+    pdf = np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    y = od.linear(x, torch.ones(1, 1, dtype=dtype, device="cuda"), activation="gelu")
+    y.backward(torch.ones_like(y))
+    off = 2.0 ** -21 * (1 + z * z)
+    check(y, z * cdf, off * np.abs(z * cdf) * (1 + U[dtype]) + rounded(z * cdf, dtype) + 2.0 ** -122, "value")
+    slope = cdf + z * pdf
+    check(x.grad, slope, off * (cdf + np.abs(z) * pdf) * (1 + U[dtype]) + 2 * rounded(slope, dtype) + 2.0 ** -122, "slope")

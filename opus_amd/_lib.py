@@ -149,9 +149,12 @@ def load():
         except OSError as e:            # missing libamdhip64 etc.
             raise ImportError(f"cannot load {LIB_PATH}: {e}") from e
         for name, (restype, argtypes) in [*SYMBOLS.items(), *DENSE_SYMBOLS.items()]:
-            fn = getattr(lib, name)
-            fn.restype = restype
-            fn.argtypes = argtypes
+            # a library of the sampling alone (an ablation build, an older one) lacks the dense operators: calling one of
+            # those says which symbol is undefined
+            fn = getattr(lib, name) if name in SYMBOLS else getattr(lib, name, None)
+            if fn is not None:
+                fn.restype = restype
+                fn.argtypes = argtypes
         _lib = lib
     return _lib
 

@@ -368,3 +368,26 @@ def test_a_tangent_is_refused(standin, name):
         y = f(leaf)
         with pytest.raises(RuntimeError, match="no tangent goes through"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_a_library_of_the_sampling_alone_loads(lib, monkeypatch, tmp_path):
+    """What csrc/abl/build.sh makes has no dense operators; the sampling works from it, a dense call names what is missing."""
+    import subprocess
+    from opus_amd import _lib, opus_dense as od
+    source, out = tmp_path / "sampling.c", tmp_path / "sampling.so"
+    source.write_text("const char *opus_msmv_strerror(int code) { return code ? \"error\" : \"ok\"; }\n"
+                      + "".join(f"int {n}(void) {{ return 0; }}\n" for n in _lib.SYMBOLS if n != "opus_msmv_strerror"))
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-o", str(out), str(source)])
+    monkeypatch.setattr(_lib, "_lib", None)
+    monkeypatch.setattr(_lib, "LIB_PATH", str(out))
+    assert _lib.load() is not lib and _lib.strerror(0) == "ok"
+    monkeypatch.setattr(od, "_check", lambda *a: None)
+    with pytest.raises(AttributeError, match="undefined symbol: opus_dense"):
+        od.dropout(torch.zeros(2, 8), 0.5, 1)
+
+
+def test_ablation_builds_have_every_source_of_the_sampling():
+    csrc = os.path.join(ROOT, "opus_amd", "csrc")
+    made = re.search(r"^MSMV = (.*)$", open(os.path.join(csrc, "Makefile")).read(), re.M).group(1).split()
+    built = re.search(r'^SRCS="(.*)"$', open(os.path.join(csrc, "abl", "build.sh")).read(), re.M).group(1).split()
+    assert sorted(built) == sorted(f"{name}.hip" for name in made)

@@ -916,3 +916,74 @@ def test_gelu_keeps_its_tail(od, dtype):
     check(y, z * cdf, off * np.abs(z * cdf) * (1 + U[dtype]) + rounded(z * cdf, dtype) + 2.0 ** -122, "value")
     slope = cdf + z * pdf
     check(x.grad, slope, off * (cdf + np.abs(z) * pdf) * (1 + U[dtype]) + 2 * rounded(slope, dtype) + 2.0 ** -122, "slope")
+
+
+# ------------------------------------------------------------------------------------------------
+# results over inputs, where include/opus_dense.h allows it
+# ------------------------------------------------------------------------------------------------
+def c_call(name, *args):
+    from opus_amd import _lib
+    lib = _lib.load()
+    assert getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("M,K,N", [(1, 72, 40), (13, 4099, 57), (256, 128, 256), (1300, 72, 1301), (70, 33, 13), (40, 8192, 61)])
+def test_linear_over_its_residual(od, dtype, M, K, N):
+    """Few rows, whole and partial tiles, r cut into shares: y in the residual's place, the same bits."""
+    from opus_amd import _lib
+    rng, kind = np.random.default_rng(M), _lib.DENSE_F32 + list(TYPES).index(dtype)
+    dtype = TYPES[dtype]
+    x, w, b, r = make(rng, dtype, M, K), make(rng, dtype, N, K, std=K ** -0.5), make(rng, dtype, N), make(rng, dtype, M, N)
+    want = od.linear(x, w, b, activation="silu", residual=r, dropout_p=0.2, seed=3, offset=1)
+    need = _lib.load().opus_dense_linear_workspace_bytes(kind, M, N, K)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    drop = _lib.DenseDropout(round(0.2 * 65536), 1, 3, None)
+    c_call("opus_dense_linear_forward", kind, x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), M, N, K,
+           _lib.DENSE_ACTIVATIONS["silu"], drop, r.data_ptr(), None, ws.data_ptr(), need)
+    assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("width", [3, 37, 256, 509, 777, 1024, 2047, 4096, 5003, 8192, 10001, 16384])
+def test_norm_over_its_inputs(od, dtype, width):
+    """y and the stream over x and block, either way round: the same bits, over more rows than the workgroups take at once."""
+    import ctypes
+    from opus_amd import _lib
+    rng, kind = np.random.default_rng(width), list(TYPES).index(dtype)
+    dtype = TYPES[dtype]
+    rows = 8200 if width == 37 else 2100 if width in (777, 5003) else 9
+    one = [make(rng, dtype, 9, width) for _ in range(2)]
+    x, h = (t.repeat(-(-rows // 9), 1)[:rows].contiguous() for t in one)
+    w, pw, g = make(rng, dtype, width), make(rng, dtype, width), make(rng, dtype, width)
+    want = od.residual_norm(x, h, w, post_weight=pw, gate=g, dropout_p=0.2, seed=3, offset=1, return_stream=True)
+    drop = _lib.DenseDropout(round(0.2 * 65536), 1, 3, None)
+    for y_over, stream_over in ((0, 1), (1, 0), (0, None), (1, None), (None, 0), (None, 1)):
+        ins = [x.clone(), h.clone()]
+        outs = [torch.empty_like(x) if i is None else ins[i] for i in (y_over, stream_over)]
+        s = _lib.DenseNorm(kind, 0, rows, width, 1, 1e-5, 1.0, ins[0].data_ptr(), ins[1].data_ptr(), w.data_ptr(), None,
+                           pw.data_ptr(), None, g.data_ptr(), ctypes.addressof(drop))
+        c_call("opus_dense_norm_forward", s, outs[0].data_ptr(), outs[1].data_ptr(), None)
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]), (y_over, stream_over)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(1, 1), (70, 13), (33, 256), (9, 70001), (5000, 7)])
+def test_dropout_over_its_inputs(od, dtype, rows, cols):
+    from opus_amd import _lib
+    rng, kind = np.random.default_rng(cols), list(TYPES).index(dtype)
+    dtype = TYPES[dtype]
+    x, r = make(rng, dtype, rows, cols), make(rng, dtype, rows, cols)
+    drop = _lib.DenseDropout(round(0.4 * 65536), 1, 3, None)
+    for residual in (None, r):
+        want = od.dropout(x, 0.4, 3, offset=1, residual=residual)
+        for over in (0, 1) if residual is not None else (0,):
+            ins = [x.clone(), None if residual is None else residual.clone()]
+            c_call("opus_dense_dropout", kind, ins[0].data_ptr(), None if ins[1] is None else ins[1].data_ptr(), rows, cols, drop,
+                   ins[over].data_ptr())
+            assert torch.equal(ins[over], want)
+    same = x.clone()                                             # x and residual the same buffer, and y too
+    want = od.dropout(x, 0.4, 3, offset=1, residual=x)
+    c_call("opus_dense_dropout", kind, same.data_ptr(), same.data_ptr(), rows, cols, drop, same.data_ptr())
+    assert torch.equal(same, want)

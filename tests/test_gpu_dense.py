@@ -3,7 +3,9 @@
 Tolerances are bounds, element by element, from the arithmetic: U[t] = eps / 2 of the output's type for its one
 rounding (plus half the smallest subnormal), and 2^-23 a step of an fp32 sum (a rounding of 2^-24, and as much again
 for what a matrix instruction may drop inside) times the sum of the terms' magnitudes."""
+import functools
 import math
+import types
 
 import numpy as np
 import pytest
@@ -987,3 +989,42 @@ def test_dropout_over_its_inputs(od, dtype, rows, cols):
     want = od.dropout(x, 0.4, 3, offset=1, residual=x)
     c_call("opus_dense_dropout", kind, same.data_ptr(), same.data_ptr(), rows, cols, drop, same.data_ptr())
     assert torch.equal(same, want)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_norm_eps(od, monkeypatch, dtype, kind, post):
+    """eps where it weighs as much as the rows' variance does.  (run_norm's bounds take 1 / sigma with 1e-5, which is an upper
+    bound for a larger eps.)  Half as much again in the oracle is seen."""
+    plain = do.residual_norm
+
+    def run(eps, oracle_eps, **kw):
+        monkeypatch.setattr(do, "residual_norm", functools.partial(plain, eps=oracle_eps))
+        run_norm(types.SimpleNamespace(residual_norm=functools.partial(od.residual_norm, eps=eps)), 60, TYPES[dtype], 3, 7, 200,
+                 kind=kind, post=post, gate="token", **kw)
+
+    run(0.3, 0.3)
+    run(2.0, 2.0, p=0.2)
+    with pytest.raises(AssertionError, match="off by"):
+        run(0.3, 0.45)
+
+
+@pytest.mark.parametrize("width", [40, 777, 2048, 5003, 16384])
+def test_norm_eps_scales_with_the_square(od, width):
+    """Rows times 2^k and eps times 4^k give the same bits, in every variant of the kernels, at both norms."""
+    rng = np.random.default_rng(width)
+    x, h = make(rng, torch.float32, 3, width), make(rng, torch.float32, 3, width)
+    w, dy = make(rng, torch.float32, width), make(rng, torch.float32, 3, width)
+
+    def run(k, eps):
+        # post's norm has to see the scaled block and hand on what x is scaled by
+        a, b, pw = x * 2.0 ** k, h * 2.0 ** k, torch.full((width,), 2.0 ** k, device="cuda")
+        leaves = [t.detach().requires_grad_(True) for t in (a, b, w, pw)]
+        y = od.residual_norm(leaves[0], leaves[1], leaves[2], post_weight=leaves[3], kind="layer", eps=eps * 4.0 ** k)
+        dx, dh, dw, dpw = torch.autograd.grad(y, leaves, dy)
+        return y, dx * 2.0 ** k, dh * 2.0 ** k, dw, dpw * 2.0 ** k
+
+    for k in (-9, 7):
+        for a, b in zip(run(0, 0.0625), run(k, 0.0625)):
+            assert torch.equal(a, b)

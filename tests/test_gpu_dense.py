@@ -1028,3 +1028,56 @@ def test_norm_eps_scales_with_the_square(od, width):
     for k in (-9, 7):
         for a, b in zip(run(0, 0.0625), run(k, 0.0625)):
             assert torch.equal(a, b)
+
+
+def test_gradients_of_sampling_and_decoder_layer_together(od):
+    """Every gradient of the step, every element.  From the sampled features on against 64 bits (a smooth activation, so that no
+    sign is open); the features' and the query's through the sampling's own backward of that gradient."""
+    from opus_amd import opus_sampling
+    from helpers import sampling4d_case, TINY_LEVELS
+    B, Q, T, G, P, N, E, S, F = 1, 60, 2, 4, 2, 6, 256, 4 * 2 * 2 * 64, 128
+    _, _, occ2img = sampling4d_case(5, B, Q, T, G, P, N=N)
+    gen = torch.Generator("cuda").manual_seed(19)
+    n = lambda *s, std=1.0: torch.randn(s, generator=gen, device="cuda") * std                    # noqa: E731
+    feats = [n(B * T * G, N, h, w, 64).requires_grad_(True) for h, w in TINY_LEVELS]
+    query = n(B, Q, E).requires_grad_(True)
+    points = torch.rand((B, Q, 8, 3), generator=gen, device="cuda")
+    ow, ob, sw, sb = n(G * P * 3, E, std=0.06), n(G * P * 3), n(G * P * 4, E, std=0.06), n(G * P * 4)
+    sp, scales = opus_sampling.sampling_inputs(points, query, ow, ob, sw, sb, T, G, P, 4, [-40.0, -40.0, -1.0, 40.0, 40.0, 5.4], fused=True)
+    out = opus_sampling.sampling_4d(sp, feats, scales, torch.from_numpy(occ2img).cuda(), 256, 704, N)
+    sampled = out.reshape(B, Q, -1)
+    t = layer_tensors(E=E, S=S, F=F)
+    names = ["w0", "b0", "g0", "h0", "w1", "b1", "w2", "b2", "g1", "h1"]
+    leaves = [t[k].requires_grad_(True) for k in names]
+
+    def dense(sampled, query, lin, norm, drop, t):
+        q = norm(query + drop(lin(sampled, t["w0"], t["b0"]), 0), t["g0"], t["h0"])
+        return norm(q + drop(lin(drop(torch.nn.functional.gelu(lin(q, t["w1"], t["b1"])), 1), t["w2"], t["b2"]), 2), t["g1"], t["h1"])
+
+    d = lambda i: dict(dropout_p=0.1, seed=33, offset=i)                                           # noqa: E731
+    q = od.residual_norm(query, od.linear(sampled, t["w0"], t["b0"]), t["g0"], t["h0"], **d(0))
+    y = od.residual_norm(q, od.linear(od.linear(q, t["w1"], t["b1"], activation="gelu", **d(1)), t["w2"], t["b2"]), t["g1"],
+                         t["h1"], **d(2))
+    grad = n(B, Q, E)
+    got = torch.autograd.grad(y, [sampled, query, *leaves, *feats], grad, retain_graph=True)
+    # the same step's parts in 64 bits
+    c = {k: v.detach().cpu().double().requires_grad_(True) for k, v in t.items()}
+    c["sampled"], c["query"] = (v.detach().cpu().double().requires_grad_(True) for v in (sampled, query))
+    keeps = [torch.from_numpy(do.keep(B * Q, w, 0.1, 33, i)).view(B, Q, w) for i, w in enumerate((E, F, E))]
+    want = dense(c["sampled"], c["query"], torch.nn.functional.linear, lambda r, g, h: torch.nn.functional.layer_norm(r, (E,), g, h),
+                 lambda v, i: keeps[i] * v, c)
+    ws, wq, *wl = torch.autograd.grad(want, [c["sampled"], c["query"], *(c[k] for k in names)], grad.cpu().double())
+    # A product of r terms is off by (r + 2) steps of the norms it multiplies, which are the root of r times a typical result;
+    # at most four such products and norms stand between a gradient and either end.
+    tol = 4 * (S + 2) * STEP * S ** 0.5
+    for k, a, b in zip(["y", "sampled", *names], [y.detach(), got[0], *got[2:]], [want.detach(), ws, *wl]):
+        assert (a.cpu().double() - b).abs().max() <= tol * b.abs().max(), k
+    # the sampling's backward is linear in what it is handed (a feature's sum of up to B Q T G P hits in another order, its
+    # weights positive), and the query's two ways add up
+    handed = got[0].view_as(out)
+    through = torch.autograd.grad(out, [query, *feats], handed, retain_graph=True)
+    sizes = torch.autograd.grad(out, feats, handed.abs())
+    for a, b, size in zip(got[-len(feats):], through[1:], sizes):
+        assert ((a - b).abs() <= 2 * B * Q * T * G * P * STEP * size).all() and b.abs().max() > 0
+    total = through[0].cpu().double() + wq
+    assert (got[1].cpu().double() - total).abs().max() <= tol * wq.abs().max() + 4 * STEP * float(through[0].abs().max())

@@ -7,9 +7,13 @@
 // wider rows take 2 to 16 waves and one LDS exchange a sum.
 //
 // Backward: r, and with a post-norm the block's normed rows, are computed again from x and block with the forward's
-// statistics.  Sums over rows (dweight, dbias, dpost_*, dgate) stay in each thread's registers while its workgroup
+// statistics.  Sums over rows (dweight, dbias, dpost_*, dgate) stay with the thread while its workgroup
 // walks a run of rows, are stored once a workgroup as fp32 rows, and a second small kernel adds those up: no atomics,
 // the same order every time.  All sums are in fp32.
+//
+// Where that is more than a thread has registers for, the compiler keeps the rest in scratch memory: in the backward above
+// 8192 elements (320 to 1312 bytes a lane), of odd widths above 4096 (36 to 652), and of whole ones there with post-norm and
+// biases (52 to 60); in the forward above 8192 in fp32 and of odd widths (44 to 244).
 //
 // Measured on one MI355X: 38400 x 256 fp32 LayerNorm with dropout 30 us forward (157 MB, 5.2 TB/s), 40 backward (236 MB,
 // 5.9 TB/s) and 6 for the sums over rows; 8192 x 8192 bf16 RMS with post-norm and a gate a sample 117 forward (537 MB,
@@ -249,9 +253,10 @@ __global__ void __launch_bounds__(group_threads(TPR)) dense_norm_backward_kernel
 {
     constexpr int ROWS = group_threads(TPR) / TPR;
     constexpr bool KEEP = sizeof(T) * VEC * CH <= 16;
-    // (not where the next row's registers would spill: 8192 x 8192 bf16 with a post-norm 337 us ahead, 376 not, but with
-    // biases as well 454 and 421; 8 elements a thread of 1024 threads instead of 16 of 512: 397 and up)
-    constexpr bool AHEAD = CH == 1 || (TPR < 1024 && sizeof(T) == 2 && !(POST && BIAS));
+    // Not where the next row's registers would spill, or spill more: 8192 x 8192 bf16 with a post-norm 337 us ahead, 376 not, but
+    // with biases as well 454 and 421; 5003 wide, whose last vectors are partial, 293 and 279 (RMS).  (Eight elements a thread
+    // of 1024 threads instead of 16 of 512: 397 and up.)
+    constexpr bool AHEAD = CH == 1 || (WHOLE && TPR < 1024 && sizeof(T) == 2 && !(POST && BIAS));
     __shared__ float lds[64];
     __shared__ __align__(16) float cols[ROWS > 1 ? ROWS * TPR * VEC : 4];
     int phase = 0;

@@ -1081,3 +1081,22 @@ def test_gradients_of_sampling_and_decoder_layer_together(od):
         assert ((a - b).abs() <= 2 * B * Q * T * G * P * STEP * size).all() and b.abs().max() > 0
     total = through[0].cpu().double() + wq
     assert (got[1].cpu().double() - total).abs().max() <= tol * wq.abs().max() + 4 * STEP * float(through[0].abs().max())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=list(TYPES))
+def test_a_training_step_repeats_bit_for_bit(od, dtype):
+    """Results and every gradient, odd sizes, all of the epilogue: the same bits from call to call."""
+    rng, dtype = np.random.default_rng(93), TYPES[dtype]
+    M, K, N = 1237, 333, 777
+    x, w, b, r = (make(rng, dtype, *s).requires_grad_(True) for s in ((M, K), (N, K), (N,), (M, N)))
+    dy = make(rng, dtype, M, N)
+
+    def step():
+        y = od.linear(x, w, b, activation="gelu", residual=r, dropout_p=0.1, seed=4)
+        n, s = od.residual_norm(y, r, b, gate=r, post_weight=b, dropout_p=0.25, seed=4, offset=1, return_stream=True)
+        return [y, n, s, *torch.autograd.grad([n, s], [x, w, b, r], [dy, dy])]
+
+    want = step()
+    for _ in range(3):
+        for p, q in zip(step(), want):
+            assert torch.equal(p, q)

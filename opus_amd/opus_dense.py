@@ -32,6 +32,7 @@ import functools
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental import proxy_tensor
 
 from . import _lib
 
@@ -121,28 +122,25 @@ def _contiguous(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
+_is_tracing, _transforms_active = torch._C._is_tracing, torch._C._are_functorch_transforms_active
+
+
 def _refuse_transforms(what, tensors):
     """A graph tracer at the dispatcher (make_fx) and functionalisation see the allocations of a call but not its kernels:
     what they make of it would return memory nobody wrote."""
-    if _dispatch_modes() or torch._ops._len_torch_dispatch_stack_pre_dispatch():
-        from torch.fx.experimental.proxy_tensor import get_proxy_mode
-        if get_proxy_mode() is not None:
-            raise RuntimeError(f"{what}: cannot be traced by torch.fx")
+    if proxy_tensor._CURRENT_MAKE_FX_TRACER is not None and proxy_tensor.get_proxy_mode() is not None:      # (this thread's)
+        raise RuntimeError(f"{what}: cannot be traced by torch.fx")
     if _transforms_active() and any(t is not None and torch._is_functional_tensor(t) for t in tensors):
         raise RuntimeError(f"{what}: cannot be functionalised")
-
-
-_tracing_state = torch._C._get_tracing_state
-_dispatch_modes = torch._C._len_torch_dispatch_stack
-_transforms_active = torch._C._are_functorch_transforms_active
 
 
 def _needs_autograd(what, tensors):
     """Whether a call has to go through its autograd function: where a gradient is wanted; under ``torch.jit.trace``, which
     records that function and not the kernels inside; and in a forward-mode level, where that function refuses a tensor
     with a tangent, which would otherwise be lost."""
-    _refuse_transforms(what, tensors)
-    if _tracing_state() is not None or forward_ad._current_level >= 0:
+    if proxy_tensor._CURRENT_MAKE_FX_TRACER is not None or _transforms_active():
+        _refuse_transforms(what, tensors)
+    if _is_tracing() or forward_ad._current_level >= 0:
         return True
     if torch.is_grad_enabled():
         for t in tensors:
@@ -159,7 +157,7 @@ def _first_order(backward):
     @functools.wraps(backward)
     def run(ctx, *grads):
         _refuse_transforms("backward", grads)
-        if _tracing_state() is not None:
+        if _is_tracing():
             raise RuntimeError("a backward of a dense operator cannot be traced")
         if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
             raise RuntimeError("gradients of a dense operator are first-order only: no tangent goes through its backward")

@@ -391,3 +391,14 @@ def test_ablation_builds_have_every_source_of_the_sampling():
     made = re.search(r"^MSMV = (.*)$", open(os.path.join(csrc, "Makefile")).read(), re.M).group(1).split()
     built = re.search(r'^SRCS="(.*)"$', open(os.path.join(csrc, "abl", "build.sh")).read(), re.M).group(1).split()
     assert sorted(built) == sorted(f"{name}.hip" for name in made)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", CALLS)
+def test_compiled_functions_break_their_graph_at_a_call(standin, name):
+    """torch.compile runs the call as it is, between what it makes of the rest."""
+    f = torch.compile(lambda x: CALLS[name](standin, x + 1) * 2, backend="aot_eager")
+    for rows in (4, 9):
+        for wants_grad in (False, True):
+            x = torch.randn(rows, 6, requires_grad=wants_grad)
+            assert torch.equal(f(x).detach(), (CALLS[name](standin, x + 1) * 2).detach())

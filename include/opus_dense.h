@@ -18,6 +18,8 @@
  *   - Outputs must not overlap inputs, except where an entry says so.
  *   - Return value: OPUS_DENSE_OK (0) or a negative OPUS_DENSE_E* code; text via opus_dense_strerror().  Arguments
  *     are checked before anything is launched; sizes of zero are no error (outputs that exist are still written).
+ *     OPUS_DENSE_ETOOLARGE may also mean that a kernel would need more threads than a launch counts (2^32), and then
+ *     come after a launch: buffers for results hold nothing of use.
  */
 #ifndef OPUS_DENSE_H
 #define OPUS_DENSE_H
@@ -68,7 +70,8 @@ const char *opus_dense_strerror(int code);
 /*
  * y = residual + D(act(x W^T + bias)) for x [M, K], W [N, K], bias [N] or NULL, residual [M, N] or NULL.
  * Products and sums are in fp32; y [M, N] is rounded once.  z [M, N] (NULL: not wanted) receives x W^T + bias in
- * the element type, which is what the backward needs where there is an activation.
+ * the element type, which is what the backward needs where there is an activation; what that type cannot hold though
+ * it is finite becomes the type's largest number of its sign.
  * y may be the same buffer as residual.
  */
 size_t opus_dense_linear_workspace_bytes(int type, long long M, long long N, long long K);

@@ -173,8 +173,9 @@ __device__ __forceinline__ float dn_silu(float z) { return z / (1.f + expf(-z));
 
 // 1 / (1 + exp(-a)), for results that are rounded to 16 bits with the hardware's exponential and reciprocal: the error is
 // within 2^-21 (1 + |a|) of the value against a half step of 2^-11 (fp16) or 2^-8 (bf16), and 0 instead of the 1e-38 that is
-// left below a = -87.  8192 x 4096 x 4096 bf16 with silu: 239 -> 223 us, with gelu_tanh 240 -> 226 us (228 without either);
-// dz of 8192 x 4096 bf16 with silu and dropout 58 -> 46 us.
+// left below a = -87.  8192 x 4096 x 4096 bf16 with silu: 225 us, 242 with expf and a division; with gelu_tanh 228 and 244
+// (221 without either); 4800 x 256 -> 18432 bf16 with silu 109 and 160 (96 without).  dz of 8192 x 4096 bf16 with silu and
+// dropout 46 and 58.
 template <class T> __device__ __forceinline__ float dn_sigmoid(float a)
 {
     if constexpr (sizeof(T) == 4)
@@ -187,8 +188,8 @@ template <class T> __device__ __forceinline__ float dn_sigmoid(float a)
 // would be off by 2 %, gelu(-5.5) be 0.  For 16-bit types Phi(-|z|) = exp(-z^2 / 2) times a polynomial in 1 / (1 + 0.26 |z|),
 // fitted to erfcx(|z| / sqrt 2) / 2 over 0 .. 15 by least squares, reweighted until the largest relative error was smallest
 // (2^-24.9; with its roundings and the hardware's exponential and reciprocal within 2^-20 (1 + z^2)).  8192 x 4096 x 4096
-// bf16 with gelu: 236 us (erff 242, erfcf 252); 4800 x 256 -> 18432 bf16: 143 (erff 169, erfcf 1.2 times that).  fp32:
-// 4800 x 256 -> 1024 48 us (erff 46).
+// bf16 with gelu: 237 us (erff 246, erfcf 256; 221 without activation); 4800 x 256 -> 18432 bf16: 146 (173, 208; 96).  fp32,
+// 4800 x 256 -> 1024: erfcf 48 us, erff 45.5.
 template <class T> __device__ __forceinline__ float dn_normal(float z, float &bell)
 {
     if constexpr (sizeof(T) == 4) {

@@ -3,7 +3,7 @@
 // A thread takes eight consecutive elements of a row, the unit one call of the generator serves; a row starts a new
 // unit, so rows of any length can be cut up.  Consecutive threads take consecutive units: 16 (32) bytes a lane.
 //
-// Measured on one MI355X: 65536 x 2048 bf16 88 us (537 MB, 6.1 TB/s; torch's copy of it 98), 38400 x 256 fp32 with a
+// Measured on one MI355X: 65536 x 2048 bf16 87 us (537 MB, 6.2 TB/s; torch's copy of it 99), 38400 x 256 fp32 with a
 // residual 18.5 us (118 MB, 6.4 TB/s).  The generator's ten rounds stay hidden behind the bytes because one call serves
 // eight elements: with nothing to drop the same kernel takes 90 and 18 us.
 #include "dense_common.h"

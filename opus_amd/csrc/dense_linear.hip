@@ -20,10 +20,10 @@
 // tiles and a long r: r is cut up over workgroups, each stores its fp32 share, and a second kernel adds the shares in
 // order and runs the epilogue.  No atomics: the result does not depend on the order of the workgroups.
 //
-// Measured on one MI355X (the library's plain products in brackets): 8192 x 4096 x 4096 bf16 forward 225 us = 1220 TFLOP/s
-// (196), dx 221 (217), dW 221 (247); 4096^3 fp32 965 us = 142 TFLOP/s; 4800 x 256 -> 18432 bf16 forward 97 (96),
-// both gradients 132 (214); 4800 x 8192 -> 256 fp32 forward 189 (228), both gradients 335 (342).  The wide tile's matrix
-// cores are busy 59 % of its cycles, LDS 24 %: without the transfers, or without the reads of LDS, it would be 15 % faster
+// Measured on one MI355X (the library's plain products in brackets, same card and run; dW with the bias' gradient):
+// 8192 x 4096 x 4096 bf16 forward 218 us = 1263 TFLOP/s (187), dx 218 (210), dW 224 (235); 4096^3 fp32 962 us = 143 TFLOP/s
+// (916); 4800 x 256 -> 18432 bf16 forward 86 (88), both gradients 130 (200); 4800 x 8192 -> 256 fp32 forward 189 (224), both
+// gradients 335 (355).  With silu and a residual the wide tile's matrix cores are busy 63 % of its cycles, LDS 26 %: without the transfers, or without the reads of LDS, it would be 15 % faster
 // each, so both have to run beside the matrix instructions, which are interleaved with them.  With few steps of r (256)
 // start and epilogue weigh as much as the product.
 #include "dense_common.h"
@@ -698,6 +698,10 @@ __global__ void __launch_bounds__(256) dense_colsum_kernel(const T *dz, long lon
 // threads a row, eight columns each; 256 >> lx rows at a time, whose sums meet in LDS; a run of rows a workgroup, which
 // the kernels above add.  8192 x 4096 bf16 with silu and dropout: 46 us (201 MB, 4.4 TB/s, beside the generator and the slope);
 // loading the next row ahead gains nothing.
+//
+// dz itself is rounded to 16 bits, and so was z before it: a 16-bit matrix instruction takes 16-bit operands, and dz in two parts
+// would double both products of the backward.  Of fp16 gradients of 1237 x 333 -> 777 with gelu and dropout, relative to 64
+// bits: 3.0e-4; z alone rounded 2.2e-4, dz alone 2.9e-4, only the results 2.1e-4.
 struct DzArgs {
     const void *dy, *z;
     void *dz;
@@ -761,7 +765,8 @@ constexpr TileKind TILES[] = {{64, 64, 4, 330, 1350}, {128, 128, 2, 800, 4700}, 
 // Which tile, and into how many shares r is cut: the cheapest by this estimate.  A CU works through its workgroups in
 // turns of as many as fit it; a step of r costs them together the cost above, and never less than the time a transfer
 // takes to arrive; a workgroup's start and end cost about as much as a few steps; shares are written, read and added by
-// a further kernel.
+// a further kernel.  Against the best of a sweep over tiles and cuts it comes within 5 % for 30 of 33 products, within 12 %
+// for two and 25 % for one (the odd 1237 x 333 -> 777's dx in 16 bits, which goes through registers: 17.2 us and 13.8).
 constexpr double ARRIVE = 1400, START_END = 8000, JOIN = 14000, JOIN_BYTES = 2000;
 
 // `only`: that kind of tile.
@@ -1001,10 +1006,11 @@ hipError_t backward(int type, const void *dz, const void *x, const void *w, long
 
 }  // namespace
 
-// Few rows take their own kernel rather than tiles (1 row, 1024 -> 4096 bf16: 4.6 us and 8.4; 16 rows, 4096 -> 4096: 11.6
-// and 14.3; 1 row, 8192 -> 8192 fp32: 52 and 85), but for two shapes: few columns over long rows of W, which leave most of
-// the chip idle (1 row, 8192 -> 256 fp32: 19.7 and 16.1), and many 16-bit rows over a large W, where reading x again for
-// every 16 columns shows (16 rows, 8192 -> 8192 bf16: 39 and 31).
+// Few rows take their own kernel rather than tiles (1 row, 1024 -> 4096 bf16: 3.5 us and 7.3; 16 rows, 4096 -> 4096: 10.3
+// and 12.8; 1 row, 8192 -> 8192 fp32: 44 and 78), but for two shapes: few columns over long rows of W, which leave most of
+// the chip idle (1 row, 8192 -> 256 fp32: 20.0 and 16.0), and many 16-bit rows over a large W, where reading x again for
+// every 16 columns shows (16 rows, 8192 -> 8192 bf16: 32 and 25).  Of 252 products measured around the limits the rule takes
+// the slower kernel for 30, by 26 % at most (8 rows, 16384 -> 2048 bf16: 25.7 and 20.4).
 static bool few_rows(int type, long long M, long long N, long long K)
 {
     if (M > FEW_ROWS)

@@ -15,10 +15,12 @@
 // 8192 elements (320 to 1312 bytes a lane), of odd widths above 4096 (36 to 652), and of whole ones there with post-norm and
 // biases (52 to 60); in the forward above 8192 in fp32 and of odd widths (44 to 244).
 //
-// Measured on one MI355X: 38400 x 256 fp32 LayerNorm with dropout 30 us forward (157 MB, 5.2 TB/s), 40 backward (236 MB,
-// 5.9 TB/s) and 6 for the sums over rows; 8192 x 8192 bf16 RMS with post-norm and a gate a sample 117 forward (537 MB,
-// 4.6 TB/s), 226 backward (805 MB, 3.6 TB/s: a row of 8192 with five gradients in flight fills a CU's registers, so only
-// one is worked on and one under way) and 11.
+// Measured on one MI355X: 38400 x 256 fp32 LayerNorm with dropout 28 us forward (157 MB, 5.6 TB/s), 40 backward (236 MB,
+// 5.9 TB/s) and 6 for the sums over rows; 8192 x 8192 bf16 RMS with post-norm and a gate a sample 110 forward (537 MB,
+// 4.9 TB/s), 215 backward (805 MB, 3.7 TB/s: a row of 8192 and its sums fill a thread's registers, so only one row is worked
+// on and one under way) and 10.  Whole steps' backwards of 8192 bf16 rows with post-norm: 8192 wide RMS 202 us, LayerNorm 262;
+// 5003 RMS 273; 10001 RMS 1879; 16384 RMS 1433, LayerNorm 1914, against 340 for that one's bytes at a copy's rate: above 8192
+// it is bound by the scratch memory.
 #include "dense_common.h"
 
 namespace {

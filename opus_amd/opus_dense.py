@@ -10,8 +10,8 @@ the feed-forward block, and the norm that follows each of them.
 
 Common to the three: tensors are fp32, bf16 or fp16, all of one type, on one GPU (CPU tensors raise); products, sums,
 statistics and the epilogue are in fp32 and every result is rounded once.  A tensor that is not contiguous is copied
-first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep no
-state and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
+first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep
+nothing but the sizes of workspaces and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
 call on the same inputs gives the same bits (asking for other gradients along with one may round that one otherwise).
 Gradients are first-order and reverse-mode only: a tensor with a forward-mode tangent is refused, before or in a backward.
 ``torch.jit.trace`` records the calls (not their backward, which raises); ``torch.fx``'s tracer at the dispatcher and
@@ -253,8 +253,9 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout_p=0.0
     x [..., K], weight [N, K], bias [N] or None, residual [..., N] or None -> [..., N].  ``activation``: "none",
     "relu", "gelu" (with erf), "gelu_tanh" or "silu".  ``dropout_p``, ``seed``, ``offset``: see the module's text.
     Gradients flow to x, weight, bias and residual.  With an activation the backward needs x W^T + bias, which the
-    forward then stores in the tensors' type (only where a gradient is wanted); d act(x W^T + bias) is rounded to that
-    type too before the two products of the backward (the bias' gradient is summed before)."""
+    forward then stores in the tensors' type (only where a gradient is wanted; finite values beyond that type as its largest
+    number); d act(x W^T + bias) is rounded to that type too before the two products of the backward (the bias' gradient is
+    summed before)."""
     args = x, weight, bias, residual, activation, dropout_p, seed, offset
     if _needs_autograd("linear", args[:4]):
         return _Linear.apply(*args)

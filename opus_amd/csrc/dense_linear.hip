@@ -23,9 +23,9 @@
 // Measured on one MI355X (the library's plain products in brackets, same card and run; dW with the bias' gradient):
 // 8192 x 4096 x 4096 bf16 forward 218 us = 1263 TFLOP/s (187), dx 218 (210), dW 224 (235); 4096^3 fp32 962 us = 143 TFLOP/s
 // (916); 4800 x 256 -> 18432 bf16 forward 86 (88), both gradients 130 (200); 4800 x 8192 -> 256 fp32 forward 189 (224), both
-// gradients 335 (355).  With silu and a residual the wide tile's matrix cores are busy 63 % of its cycles, LDS 26 %: without the transfers, or without the reads of LDS, it would be 15 % faster
-// each, so both have to run beside the matrix instructions, which are interleaved with them.  With few steps of r (256)
-// start and epilogue weigh as much as the product.
+// gradients 335 (355).  With silu and a residual the wide tile's matrix cores are busy 63 % of its cycles, LDS 26 %: without
+// the transfers, or without the reads of LDS, it would be 15 % faster each, so both have to run beside the matrix
+// instructions, which are interleaved with them.  With few steps of r (256) start and epilogue weigh as much as the product.
 #include "dense_common.h"
 
 namespace {

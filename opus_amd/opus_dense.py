@@ -10,9 +10,11 @@ the feed-forward block, and the norm that follows each of them.
 
 Common to the three: tensors are fp32, bf16 or fp16, all of one type, on one GPU (CPU tensors raise); products, sums,
 statistics and the epilogue are in fp32 and every result is rounded once.  A tensor that is not contiguous is copied
-first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep
-nothing but the sizes of workspaces and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run: the same
-call on the same inputs gives the same bits (asking for other gradients along with one may round that one otherwise).
+first.  The calls are asynchronous on the current stream of the tensors' device, allocate through torch, keep nothing but
+the sizes of workspaces and can be captured into a HIP graph.  Results do not depend on the order in which workgroups run:
+the same call on the same inputs gives the same bits (asking for other gradients along with one may round that one
+otherwise).
+
 Gradients are first-order and reverse-mode only: a tensor with a forward-mode tangent is refused, before or in a backward.
 ``torch.jit.trace`` records the calls (not their backward, which raises); ``torch.fx``'s tracer at the dispatcher and
 ``torch.func``'s transforms are refused.
@@ -215,7 +217,8 @@ def _linear_forward(x, weight, bias, residual, activation, dropout_p, seed, offs
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, dropout_p, seed, offset):
-        y, z, code, drop = _linear_forward(x, weight, bias, residual, activation, dropout_p, seed, offset, True)
+        y, z, code, drop = _linear_forward(x, weight, bias, residual, activation, dropout_p, seed, offset,
+                                           any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, z, _seed_tensor(drop, seed))
         ctx.settings = code, drop
         return y

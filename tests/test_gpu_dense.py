@@ -1100,3 +1100,29 @@ def test_a_training_step_repeats_bit_for_bit(od, dtype):
     for _ in range(3):
         for p, q in zip(step(), want):
             assert torch.equal(p, q)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_a_traced_module_trains(od):
+    """Results and gradients of a traced module for other shapes and another seed tensor, and its results without gradients."""
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.Parameter(torch.randn(24, 16, device="cuda"))
+            self.g = torch.nn.Parameter(torch.randn(24, device="cuda"))
+
+        def forward(self, x, seed):
+            h = od.linear(x, self.w, activation="gelu", dropout_p=0.3, seed=seed)
+            return od.residual_norm(h, h, self.g, gate=h, dropout_p=0.2, seed=seed, offset=1)
+
+    m = Block()
+    traced = torch.jit.trace(m, (torch.randn(5, 7, 16, device="cuda"), torch.tensor([3], device="cuda")))
+    for i, shape in enumerate(((5, 7, 16), (2, 3, 16), (9, 16))):
+        x, seed = torch.randn(shape, device="cuda", requires_grad=True), torch.tensor([i], device="cuda")
+        want, got = m(x, seed), traced(x, seed)
+        dy = torch.randn_like(want)
+        assert torch.equal(got, want)
+        for a, b in zip(*(torch.autograd.grad(y, [x, m.w, m.g], dy) for y in (got, want))):
+            assert torch.equal(a, b)
+        with torch.no_grad():
+            assert torch.equal(traced(x, seed), want)
